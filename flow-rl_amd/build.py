@@ -23,9 +23,12 @@ CSRC = HERE / "csrc"
 OBJ = CSRC / "_obj"
 OUT = HERE / "flowrl_hip" / "libflowrl_hip.so"
 ARCH = "gfx950"
+NO_PACKED = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # (source, object stem, extra defines); the register-streamed sampler is one translation unit per activation
 SOURCES = [("capi.hip", "capi", []), ("prepare.hip", "prepare", []),
            ("cond_embed.hip", "cond_embed", []), ("critic_select.hip", "critic_select", []), ("time_bwd.hip", "time_bwd", []), ("rng.hip", "rng", []), ("net_eval.hip", "net_eval", []), ("net_vjp_layered.hip", "net_vjp_layered", []),
+           # rows of logits: scalar float32 throughout (the packed forms buy a memory-bound kernel nothing)
+           ("logits.hip", "logits", NO_PACKED), ("distill.hip", "distill", NO_PACKED),
            ("sampler_bf16.hip", "sampler_bf16", ["-fno-slp-vectorize"]),
            ] + [("sampler_bwd_bf16.hip", f"sampler_bwd_bf16_p{p}", ["-fno-slp-vectorize", f"-DFRL_BWD16_PHASE={p}"]) for p in range(3)] + \
           [("sampler_bwd.hip", f"sampler_bwd_p{p}", [f"-DFRL_BWD_PHASE={p}"]) for p in range(3)] + [("sampler_bwd_lat.hip", "sampler_bwd_lat", [])] + \
@@ -33,6 +36,7 @@ SOURCES = [("capi.hip", "capi", []), ("prepare.hip", "prepare", []),
           [("sampler_res.hip", f"sampler_res_act{a}", [f"-DFRL_RES_ACT={a}"]) for a in range(6)] + \
           [("sampler_lat.hip", f"sampler_lat_act{a}", [f"-DFRL_RS_ACT={a}"]) for a in range(7)]   # 6 = identity: the post-activation-LayerNorm units
 HEADERS = [CSRC / "frl_internal.h", CSRC / "frl_device.h", CSRC / "frl_bf16.h", CSRC / "frl_rng.h", CSRC / "frl_actgrad.h", ROOT / "include" / "flowrl_hip.h"]
+EXTRA_HEADERS = {"logits.hip": [CSRC / "frl_rows.h"], "distill.hip": [CSRC / "frl_rows.h"]}
 FLAGS = ["-O3", "-fPIC", f"--offload-arch={ARCH}", "-std=c++17", "-Wno-unused-value",
          f"-I{ROOT / 'include'}", f"-I{CSRC}"]
 
@@ -60,7 +64,7 @@ def build(force: bool = False, jobs: int = 8, verbose: bool = True) -> Path:
         s = CSRC / src
         o = OBJ / (stem + ".o")
         objs.append(o)
-        if force or _stale(o, [s, *HEADERS, Path(__file__)]):
+        if force or _stale(o, [s, *HEADERS, *EXTRA_HEADERS.get(src, []), Path(__file__)]):
             todo.append((s, o, defs))
 
     def compile_one(so):

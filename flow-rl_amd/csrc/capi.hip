@@ -47,7 +47,7 @@ void set_error(const char* fmt, ...) {
 }
 
 static thread_local char g_kern[1024] = "";
-static void clear_kernels() { g_kern[0] = 0; }
+void clear_kernels() { g_kern[0] = 0; }
 void note_kernel(const char* fmt, ...) {
   const size_t n = strlen(g_kern);
   if (n + 4 >= sizeof(g_kern)) return;

@@ -97,6 +97,39 @@ class FrlEvalBwdBufs(C.Structure):
                 ("grad_final_ln_scale", _fp), ("grad_final_ln_bias", _fp)]
 
 
+FRL_ELT_F32, FRL_ELT_BF16, FRL_ELT_F16 = 0, 1, 2
+FRL_MASK_NONE, FRL_MASK_WORDS, FRL_MASK_BYTES = 0, 1, 2
+FRL_DISTILL_TOP, FRL_DISTILL_REST = 0, 1
+FRL_REDUCE_NONE, FRL_REDUCE_SUM, FRL_REDUCE_MEAN = 0, 1, 2
+FRL_LOGITS_MAX_SPARSE, FRL_DISTILL_MAX_TOP, FRL_DISTILL_STATS = 2048, 1024, 4
+
+
+class FrlLogitsDesc(C.Structure):
+    _fields_ = [("abi_version", C.c_int32), ("dtype", C.c_int32), ("out_dtype", C.c_int32), ("vocab", C.c_int32), ("rows", C.c_int64),
+                ("ids64", C.c_int32), ("history_len", C.c_int32), ("n_sparse", C.c_int32), ("mask", C.c_int32),
+                ("logits_stride", C.c_int64), ("out_stride", C.c_int64), ("gumbel_stride", C.c_int64), ("history_stride", C.c_int64),
+                ("bias_stride", C.c_int64), ("sparse_stride", C.c_int64), ("mask_stride", C.c_int64),
+                ("repetition", C.c_float), ("frequency", C.c_float), ("presence", C.c_float), ("temperature", C.c_float)]
+
+
+class FrlLogitsBufs(C.Structure):
+    _fields_ = [("logits", _fp), ("out", _fp), ("history", _fp), ("lengths", _fp), ("prompt_lengths", _fp), ("repetition", _fp),
+                ("frequency", _fp), ("presence", _fp), ("bias", _fp), ("bias_tokens", _fp), ("bias_values", _fp), ("allowed", _fp),
+                ("temperature", _fp), ("gumbel", _fp), ("token", _fp), ("logprob", _fp)]
+
+
+class FrlDistillDesc(C.Structure):
+    _fields_ = [("abi_version", C.c_int32), ("dtype", C.c_int32), ("teacher_dtype", C.c_int32), ("ids64", C.c_int32), ("kind", C.c_int32),
+                ("reduction", C.c_int32), ("vocab", C.c_int32), ("top", C.c_int32), ("rows", C.c_int64),
+                ("logits_stride", C.c_int64), ("grad_stride", C.c_int64), ("ids_stride", C.c_int64), ("teacher_stride", C.c_int64),
+                ("temperature", C.c_float)]
+
+
+class FrlDistillBufs(C.Structure):
+    _fields_ = [("logits", _fp), ("ids", _fp), ("teacher", _fp), ("weights", _fp), ("loss", _fp), ("row_stats", _fp), ("g_loss", _fp),
+                ("grad", _fp)]
+
+
 FRL_NOISE_DDPM, FRL_NOISE_CDDPM_LINEAR, FRL_NOISE_CDDPM_COSINE, FRL_NOISE_FLOW = 0, 1, 2, 3
 FRL_MSE_WORKSPACE_BYTES = 2048
 
@@ -159,6 +192,12 @@ EXPORTS = {
     "frl_ddpm_onestep_update": (C.c_int, [C.c_int32, C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                           C.c_void_p, C.c_int32, C.c_int32, C.c_float, C.c_float, C.c_void_p, C.c_void_p, C.c_void_p]),
     "frl_mse_loss": (C.c_int, [C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "frl_logits_constrain": (C.c_int, [C.POINTER(FrlLogitsDesc), C.POINTER(FrlLogitsBufs), C.c_void_p]),
+    "frl_logits_workspace_bytes": (C.c_size_t, [C.POINTER(FrlLogitsDesc)]),
+    "frl_logits_choose": (C.c_int, [C.POINTER(FrlLogitsDesc), C.POINTER(FrlLogitsBufs), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "frl_distill_workspace_bytes": (C.c_size_t, [C.POINTER(FrlDistillDesc)]),
+    "frl_distill_fwd": (C.c_int, [C.POINTER(FrlDistillDesc), C.POINTER(FrlDistillBufs), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "frl_distill_bwd": (C.c_int, [C.POINTER(FrlDistillDesc), C.POINTER(FrlDistillBufs), C.c_void_p]),
     "frl_selftest_mfma32": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
 }
 

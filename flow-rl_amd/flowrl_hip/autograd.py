@@ -23,6 +23,7 @@ from typing import Callable, Dict, List, Optional, Tuple
 
 import torch
 
+from . import logits as _logits
 from .flow.cnf import ContinuousNormalizingFlow
 
 Path = Tuple[str, ...]
@@ -137,6 +138,35 @@ def apply(model, x: torch.Tensor, t: torch.Tensor, condition: Optional[torch.Ten
     if not (torch.is_grad_enabled() and (x.requires_grad or any(leaf.requires_grad for _, leaf in flat))):
         return model(x, t, condition, True, p, particles=particles)      # nothing to differentiate: the plain evaluation
     return _ApplyFn.apply(model, t, condition, particles, [path for path, _ in flat], x, *[leaf for _, leaf in flat])
+
+
+class _DistillFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, ids, teacher, weights, kind, temperature, reduction):
+        loss, _, stats = _logits.distill_forward(logits, ids, teacher, kind, temperature, weights, reduction, want_stats=True)
+        ctx.how, ctx.stats = (kind, temperature, reduction), stats
+        ctx.save_for_backward(logits, ids, teacher, *([] if weights is None else [weights]))     # version-counter checks, as in _SampleFn
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_loss):
+        logits, ids, teacher, *w = ctx.saved_tensors
+        kind, temperature, reduction = ctx.how
+        grad = _logits.distill_backward(logits, ids, teacher, kind, temperature, w[0] if w else None, reduction, ctx.stats, g_loss)
+        return grad, None, None, None, None, None, None
+
+
+def distill_loss(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor, *, kind: str = "logits", temperature: float = 1.0,
+                 weights: Optional[torch.Tensor] = None, reduction: str = "mean") -> torch.Tensor:
+    """:func:`flowrl_hip.logits.distill_loss` as a differentiable torch op: the backward is one pass over the logits from the row statistics the
+    forward kept (frl_distill_bwd).  Gradients flow to ``logits``; the teacher and the weights are not differentiated and asking
+    for it raises."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (teacher, weights)):
+        raise NotImplementedError("flowrl_hip.autograd: distill_loss differentiates the student's logits only; detach teacher / weights")
+    if not (torch.is_grad_enabled() and logits.requires_grad):
+        return _logits.distill_loss(logits, ids, teacher, kind=kind, temperature=temperature, weights=weights, reduction=reduction)
+    return _DistillFn.apply(logits, ids, teacher, weights, kind, float(temperature), reduction)
 
 
 def value_and_grad(loss_fn: Callable, params: Dict, has_aux: bool = False):

@@ -22,7 +22,7 @@ from typing import Dict, Optional, Tuple
 
 import torch
 
-from . import _lib
+from . import _lib, logits
 from ._sampler import _f32c, _workspace
 from .module import MLP, _dense, tree_to
 
@@ -106,10 +106,12 @@ def _critic_marshal(critic: Ensemblize, params: Dict, obs: Optional[torch.Tensor
 
 def critic_select(critic: Ensemblize, params: Dict, obs: Optional[torch.Tensor], actions: torch.Tensor, num_samples: int,
                   *, temperature: Optional[float] = 0.0, gumbel: Optional[torch.Tensor] = None,
-                  want_q: bool = True) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
+                  want_q: bool = True, allowed: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
     """``obs`` (B, S) UN-repeated, ``actions`` (B, N, A) or (B*N, A).  Returns (best actions (B, A), idx (B,) int32,
     qs (B, N) = min over the ensemble).  temperature <= 0: argmax (dql.py:156-157); temperature > 0: the categorical
-    draw of dql.py:158-160 as argmax(qs / (1e-6 + T) + gumbel) with ``gumbel`` (B, N) supplied by the caller."""
+    draw of dql.py:158-160 as argmax(qs / (1e-6 + T) + gumbel) with ``gumbel`` (B, N) supplied by the caller.
+    ``allowed`` (no counterpart in the reference): which candidates may be chosen, as :class:`flowrl_hip.logits.Constraints` takes it
+    (bool (B, N), or int32 words); a state whose candidates are all ruled out answers idx -1 and an action of NaN."""
     lib = _lib.load()
     if not actions.is_cuda:
         raise RuntimeError("flowrl_hip critic scoring runs on the GPU only; there is no CPU fallback")
@@ -119,6 +121,16 @@ def critic_select(critic: Ensemblize, params: Dict, obs: Optional[torch.Tensor],
     B = actions.numel() // (A * N)
     if B * N * A != actions.numel():
         raise ValueError("actions do not hold num_samples candidates per state")
+    if allowed is not None:
+        drawn = temperature is not None and temperature > 0.0
+        if drawn and gumbel is None:
+            raise ValueError("temperature > 0 draws from a categorical: pass gumbel=(B, N) Gumbel(0,1) noise")
+        _, _, q = critic_select(critic, params, obs, actions, N)
+        idx, _ = logits.choose(q, logits.Constraints(allowed=allowed), temperature=float(temperature) if drawn else 0.0,
+                               gumbel=gumbel.reshape(B, N) if drawn else None)
+        some = (idx >= 0)[:, None]
+        best = torch.where(some, actions.reshape(B, N, A).gather(1, idx.long().clamp(min=0)[:, None, None].expand(B, 1, A))[:, 0], torch.nan)
+        return best, idx, (q if want_q else None)
     d, fp, bufs, keep, (best, idx, q) = _critic_marshal(critic, params, obs, B, N, A, dev, temperature, gumbel, want_q)
     act2 = _f32c(actions.reshape(B * N, A), dev, "actions")
     bufs.actions = act2.data_ptr()
@@ -155,7 +167,7 @@ class FusedSelect:
 def sample_and_select(model, critic: Ensemblize, critic_params: Dict, rng, obs: torch.Tensor, training: bool, num_samples: int,
                       solver: str, temperature: Optional[float], *, xT: Optional[torch.Tensor] = None,
                       noise: Optional[torch.Tensor] = None, gumbel: Optional[torch.Tensor] = None, compute_dtype: str = "f32",
-                      rng_impl: Optional[str] = None, fused="auto"):
+                      rng_impl: Optional[str] = None, fused="auto", allowed: Optional[torch.Tensor] = None):
     """jit_sample_and_select (dql.py:130-162): num_samples chains per observation, then the critic picks one.
     With a threefry key as ``rng`` (flowrl_hip.random.PRNGKey) the call is the reference's rng-in / rng-out protocol,
     all on the GPU: ``rng, xT_rng = split(rng)``; ``xT = normal(xT_rng, (B, N, A))``; the sampler draws its noise
@@ -165,7 +177,8 @@ def sample_and_select(model, critic: Ensemblize, critic_params: Dict, rng, obs: 
     ``fused``: True = one launch for sampler + critic + selection (frl_sampler_select_fwd; raises when the configuration
     has no such build), False = sampler launch, critic launches, selection launch; "auto" = fused when the build exists
     and the batch is throughput-sized (>= FUSED_MIN_CHAINS chains), else the separate launches (whose small-batch
-    latency builds the fused kernel does not have).  The fused path needs caller-side draws (no threefry key)."""
+    latency builds the fused kernel does not have).  The fused path needs caller-side draws (no threefry key).
+    ``allowed``: which of the candidates may be chosen (:func:`critic_select`); the separate launches only."""
     from . import random as fr
     B = obs.shape[0]
     keyed = fr.is_key(rng)
@@ -183,9 +196,11 @@ def sample_and_select(model, critic: Ensemblize, critic_params: Dict, rng, obs: 
     if solver is not None:
         kw["solver"] = solver
     kw = {k: v for k, v in kw.items() if k in accepted}
-    can_fuse = temperature is not None and not keyed and compute_dtype == "f32" and (temperature <= 0.0 or gumbel is not None)
+    if allowed is not None and temperature is None:
+        raise ValueError("allowed: without a temperature the first candidate is taken, not the best")
+    can_fuse = allowed is None and temperature is not None and not keyed and compute_dtype == "f32" and (temperature <= 0.0 or gumbel is not None)
     if fused is True and not can_fuse:
-        raise _lib.FlowRLHipUnsupported(_lib.FRL_EUNSUPPORTED, "fused sample+select: needs a temperature, caller-side draws (no threefry key, gumbel given) and f32")
+        raise _lib.FlowRLHipUnsupported(_lib.FRL_EUNSUPPORTED, "fused sample+select: needs a temperature, caller-side draws (no threefry key, gumbel given), f32 and no `allowed`")
     if can_fuse and (fused is True or (fused == "auto" and B * num_samples >= FUSED_MIN_CHAINS)):
         sel = FusedSelect(critic, critic_params, obs, temperature=temperature, gumbel=gumbel)
         try:
@@ -201,5 +216,5 @@ def sample_and_select(model, critic: Ensemblize, critic_params: Dict, rng, obs: 
         rng, select_rng = fr.split(rng, 2, rng_impl)                                                     # dql.py:159
         if gumbel is None:
             gumbel = fr.gumbel(select_rng, (B, num_samples), rng_impl)                                   # categorical, dql.py:160
-    best, _, _ = critic_select(critic, critic_params, obs, actions, num_samples, temperature=temperature, gumbel=gumbel, want_q=False)
+    best, _, _ = critic_select(critic, critic_params, obs, actions, num_samples, temperature=temperature, gumbel=gumbel, want_q=False, allowed=allowed)
     return rng, best

@@ -460,6 +460,123 @@ int frl_ddpm_onestep_update(int32_t solver, int64_t B, int32_t A, int32_t num_sa
 int frl_mse_loss(int64_t n, const float* pred, const float* target, float* loss, float* grad, void* workspace, size_t workspace_bytes,
                  void* hip_stream);
 
+/* ---- rows of logits over a vocabulary of discrete choices ------------------------------------------------------------
+ * No counterpart in the reference: its discrete answers stop at the critic's best-of-N (frl_critic_select), an argmax or
+ * categorical over a handful of unconstrained candidates.  These entry points choose among any number of entries (candidate
+ * actions, action tokens, a text vocabulary) under rules, and train a student on a teacher's best entries.
+ *
+ * Rows are `vocab` contiguous elements, `*_stride` elements apart; any alignment.  Element types: FRL_ELT_*.  Arithmetic
+ * is float32, each operation rounded on its own, in this order (x = logits[r][v]; c = how often v stands in the generated
+ * part of the row's history; seen = v stands anywhere in it):
+ *     seen:   x = x > 0 ? x / repetition : x * repetition
+ *             x = x - (frequency * c + (c > 0 ? presence : 0))
+ *             x = x + bias[v];  x = x + (the bias_values whose bias_tokens are v, summed in their order)
+ *     v not allowed:  x = -inf   (whatever stood there, NaN included)
+ * The history is row r of `history` up to lengths[r] (clamped to [0, history_len]); its first prompt_lengths[r] entries are
+ * the prompt: seen, not generated.  Tokens outside [0, vocab) in the lists are padding and do nothing. */
+#define FRL_ELT_F32 0
+#define FRL_ELT_BF16 1
+#define FRL_ELT_F16 2
+
+#define FRL_MASK_NONE 0
+#define FRL_MASK_WORDS 1 /* int32 words: bit v & 31 of word v >> 5 set = allowed */
+#define FRL_MASK_BYTES 2 /* one byte per entry, non-zero = allowed (a bool tensor) */
+
+#define FRL_LOGITS_MAX_SPARSE 2048 /* entries of one row's bias_tokens list; more than that is a dense bias */
+
+typedef struct FrlLogitsDesc {
+  int32_t abi_version; /* FRL_ABI_VERSION */
+  int32_t dtype;       /* FRL_ELT_* of logits */
+  int32_t out_dtype;   /* frl_logits_constrain: FRL_ELT_F32, or dtype */
+  int32_t vocab;       /* entries per row */
+  int64_t rows;
+  int32_t ids64;       /* 1: history and bias_tokens hold int64, 0: int32 */
+  int32_t history_len; /* columns of history; 0 = no history */
+  int32_t n_sparse;    /* columns of bias_tokens / bias_values; 0 = none */
+  int32_t mask;        /* FRL_MASK_*: what `allowed` holds */
+  int64_t logits_stride, out_stride, gumbel_stride, history_stride;
+  int64_t bias_stride, sparse_stride, mask_stride; /* 0: one row of them for every row of logits */
+  float repetition, frequency, presence, temperature; /* used where the per-row pointer is NULL */
+} FrlLogitsDesc;
+
+typedef struct FrlLogitsBufs {
+  const void* logits;             /* (rows, vocab) */
+  void* out;                      /* (rows, vocab); constrain only.  May be `logits` itself (same type and stride) */
+  const void* history;            /* (rows, history_len) tokens */
+  const int32_t* lengths;         /* (rows,) or NULL: every row is full */
+  const int32_t* prompt_lengths;  /* (rows,) or NULL: no prompt */
+  const float* repetition;        /* (rows,) or NULL; > 0 */
+  const float* frequency;         /* (rows,) or NULL */
+  const float* presence;          /* (rows,) or NULL */
+  const float* bias;              /* (rows | 1, vocab) or NULL */
+  const void* bias_tokens;        /* (rows | 1, n_sparse) */
+  const float* bias_values;       /* (rows | 1, n_sparse) */
+  const void* allowed;            /* (rows | 1, ceil(vocab / 32)) words or (rows | 1, vocab) bytes */
+  const float* temperature;       /* choose: (rows,) or NULL */
+  const float* gumbel;            /* choose: (rows, vocab) finite Gumbel(0, 1) noise, or NULL: every row is greedy */
+  int32_t* token;                 /* choose: (rows,) */
+  float* logprob;                 /* choose: (rows,) or NULL */
+} FrlLogitsBufs;
+
+/* out = the constrained logits, rounded once to out_dtype. */
+int frl_logits_constrain(const FrlLogitsDesc* desc, const FrlLogitsBufs* bufs, void* hip_stream);
+
+/* One entry per row of the constrained logits, without writing them.  With T = temperature > 0 and noise: y = x * (1 /
+ * (1e-6 + T)) and token = argmax(y + gumbel), the categorical draw of frl_critic_select; else y = x and token = argmax(y).
+ * The first of equal maxima; a NaN counts as the largest value (argmax's rule in jax and torch).  logprob = y[token] -
+ * log sum exp y.  A row that its rules leave nothing (every y is -inf) answers token -1, logprob -inf. */
+size_t frl_logits_workspace_bytes(const FrlLogitsDesc* desc);
+int frl_logits_choose(const FrlLogitsDesc* desc, const FrlLogitsBufs* bufs, void* workspace, size_t workspace_bytes, void* hip_stream);
+
+/* KL divergence of a student's distribution from a teacher's top entries.  q = softmax(logits[r] / temperature) over the
+ * whole vocabulary; the teacher names `top` entries of a row, ids outside [0, vocab) are padding:
+ *   FRL_DISTILL_TOP   teacher holds logits:  p = softmax(teacher / temperature) over the named entries;
+ *                     L[r] = sum p (log p - log q)
+ *   FRL_DISTILL_REST  teacher holds log-probabilities (at the temperature meant): p = exp(teacher), and the mass it leaves
+ *                     unnamed, P = 1 - sum p, is one more class of which the student has Q = the sum of q over the others:
+ *                     L[r] = sum p (log p - log q) + P log(P / Q)          (the last term only where P > 0)
+ * A token named twice counts as two entries (their p add up in the gradient; Q leaves it out once).  A row that names
+ * nothing under FRL_DISTILL_TOP, and a row of weight 0 (never read), have L = 0 and gradient 0.
+ *   loss, FRL_REDUCE_NONE: (rows,) weights[r] L[r];  FRL_REDUCE_SUM: their sum;  FRL_REDUCE_MEAN: their sum / the sum of the
+ *   weights (0 when that is 0).  Sums over rows run in a fixed order in float64. */
+#define FRL_DISTILL_TOP 0
+#define FRL_DISTILL_REST 1
+#define FRL_REDUCE_NONE 0
+#define FRL_REDUCE_SUM 1
+#define FRL_REDUCE_MEAN 2
+#define FRL_DISTILL_MAX_TOP 1024
+#define FRL_DISTILL_STATS 4 /* floats per row of row_stats */
+
+typedef struct FrlDistillDesc {
+  int32_t abi_version;   /* FRL_ABI_VERSION */
+  int32_t dtype;         /* FRL_ELT_* of logits and grad */
+  int32_t teacher_dtype; /* FRL_ELT_* of teacher */
+  int32_t ids64;         /* 1: ids are int64, 0: int32 */
+  int32_t kind;          /* FRL_DISTILL_* */
+  int32_t reduction;     /* FRL_REDUCE_* */
+  int32_t vocab, top;
+  int64_t rows;
+  int64_t logits_stride, grad_stride, ids_stride, teacher_stride;
+  float temperature; /* > 0 */
+} FrlDistillDesc;
+
+typedef struct FrlDistillBufs {
+  const void* logits;   /* (rows, vocab) */
+  const void* ids;      /* (rows, top) */
+  const void* teacher;  /* (rows, top) */
+  const float* weights; /* (rows,) or NULL: 1 */
+  float* loss;          /* fwd: scalar, or (rows,) for FRL_REDUCE_NONE */
+  float* row_stats;     /* (rows + 1, FRL_DISTILL_STATS): fwd writes it (NULL: not wanted), bwd reads it */
+  const float* g_loss;  /* bwd: dL/d loss, scalar or (rows,) */
+  void* grad;           /* (rows, vocab), dtype: bwd's result; fwd with grad != NULL also writes d loss / d logits in the same
+                           call (FRL_REDUCE_NONE: of the rows' sum).  Must not overlap logits */
+} FrlDistillBufs;
+
+size_t frl_distill_workspace_bytes(const FrlDistillDesc* desc);
+int frl_distill_fwd(const FrlDistillDesc* desc, const FrlDistillBufs* bufs, void* workspace, size_t workspace_bytes, void* hip_stream);
+/* The gradient from what the forward kept (row_stats) for the same desc, logits, ids, teacher and weights. */
+int frl_distill_bwd(const FrlDistillDesc* desc, const FrlDistillBufs* bufs, void* hip_stream);
+
 int frl_abi_version(void);
 
 /* Hardware self-test of the MFMA operand / accumulator lane maps the kernel relies on:
