@@ -251,9 +251,8 @@ def _plain_distill(s):
 # ---- the framework's calls -----------------------------------------------------------------------------------------------
 
 def _framework():
-    at = str(Path(__file__).resolve().parent.parent / "flow-rl_amd")
-    if at not in sys.path:
-        sys.path.insert(0, at)
+    if "flowrl_hip" not in sys.modules:
+        sys.path.insert(0, str(Path(__file__).resolve().parent.parent / "flow-rl_amd"))
     import flowrl_hip
     return flowrl_hip
 
