@@ -7,13 +7,14 @@
 //     dL/dz  = k q / T            the others, k = 1 (FRL_DISTILL_TOP) or 1 - P s / r (FRL_DISTILL_REST with P > 0)
 // The gradient is therefore one scaled exponential per element plus a correction of `top` elements.
 //
-// HBM-bound for long rows: the logits once, the gradient once.  A group of threads (a wave or a workgroup) takes a whole row:
-// maximum and sum in one pass, the teacher's entries beside it, then the gradient in a second pass whose reads come from the cache.
-// Few rows are split over their length, joined by a second kernel, and differentiated by a third.
+// HBM-bound for long rows: the logits once, the gradient once.  A row lives in the registers of the threads that share it (a wave up to a
+// workgroup of 1024, at most 16 vectors of 16 bytes each: 131072 entries of two bytes), so the gradient needs no second read.  With q
+// bounded by quarter-rate exponentials (four issue slots each) the rest of the arithmetic is kept to four slots per element: the shift
+// by the maximum is one fma, two bytes are packed by one convert, and the factor of a two-byte gradient goes into the exponent.
+// Rows beyond that, or too few to fill the chip, are split over their length, joined by a second kernel, and differentiated by a third.
 #include "frl_rows.h"
 
-// The value-and-gradient kernels and the backward kernel share the code below and agree bit for bit: no product is fused into a sum
-// in one of them and not in the other.
+// No product is fused into a sum but where the code says so: the kernels that share the code below then round alike.
 #pragma clang fp contract(off)
 
 namespace frl {
@@ -31,17 +32,8 @@ struct DistillArgs {
   int vocab, top, ids64, teacher_dtype, segs, seg_len, g_stride;
 };
 
-constexpr int DSEG_MAX = 1 << 18;      // entries whose named bits one workgroup keeps in LDS (32 KB)
-
-template <typename T>
-__device__ __forceinline__ f32x4 quad(const T* p, int left) {
-  if (left >= 4) return Elt<T>::load4(p);
-  f32x4 v = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-  if (left > 0) v[0] = Elt<T>::get(p[0]);
-  if (left > 1) v[1] = Elt<T>::get(p[1]);
-  if (left > 2) v[2] = Elt<T>::get(p[2]);
-  return v;
-}
+constexpr int DSEG_MAX = 1 << 16;      // entries of a segment
+constexpr int DROW_MAX = 1 << 18;      // entries of a row that is not split
 
 __device__ __forceinline__ float teacher_at(const void* p, long long i, int dtype) {
   if (dtype == FRL_ELT_F32) return ((const float*)p)[i];
@@ -61,53 +53,112 @@ __device__ __forceinline__ void mark_named(const DistillArgs& a, long long row, 
   group_sync<G>();
 }
 
-// m, s, r of entries [v0, v0 + n) of a row over the group's threads.  Each thread keeps its own running maximum and rescales
-// its sums when a batch of 16 entries raises it.
-template <typename T, int G, bool REST>
-__device__ __forceinline__ void row_sums(const T* z, int n, float c, const unsigned* words, int tid, float* red0, float* red1, float& m, float& s, float& r) {
-  constexpr int U = 4;
-  float mt = -INFINITY, st = 0.0f, rt = 0.0f;
-  for (int v = 4 * tid; v < n; v += 4 * U * G) {
-    f32x4 x[U];
+// 2^((x - m) c).  With a finite product M = m c this is one fma, whose rounding of M shifts every exponent of the row alike; a maximum near
+// the type's lowest value (a row masked throughout) takes the difference first.
+struct Shift {
+  float m, M, c;
+  bool fast;
+  __device__ __forceinline__ Shift(float m_, float c_) : m(m_), M(m_ * c_), c(c_) { fast = fabsf(M) < INFINITY; }
+  template <int N>
+  __device__ __forceinline__ void exps(float* x) const {
+    if (fast) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int at = v + 4 * G * u;
-      x[u] = quad(z + at, n - at);
+      for (int i = 0; i < N; ++i) x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], c, -M));
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = __builtin_amdgcn_exp2f((x[i] - m) * c);
     }
-    float bm = mt;
+  }
+};
+
+template <int N>
+__device__ __forceinline__ float max_of(const float* x, float m) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) bm = fmaxf(bm, fmaxf(fmaxf(x[u][0], x[u][1]), fmaxf(x[u][2], x[u][3])));
-    const float m0 = bm == -INFINITY ? 0.0f : bm;
-    const float f = __builtin_amdgcn_exp2f((mt - m0) * c);
-    st *= f;
-    rt *= f;
-    mt = bm;
+  for (int i = 0; i < N; i += 2) m = fmaxf(fmaxf(x[i], x[i + 1]), m);      // v_max3_f32
+  return m;
+}
+template <int N>
+__device__ __forceinline__ float sum_of(const float* e) {
+  float s = 0.0f;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int at = v + 4 * G * u;
-      unsigned named = 0;
-      if (REST && at < n) named = words[at >> 5] >> (at & 31);
+  for (int i = 0; i < N; ++i) s += e[i];
+  return s;
+}
+// the named bits of the N entries from v (a multiple of N)
+template <int N>
+__device__ __forceinline__ unsigned named_bits(const unsigned* words, int v) { return (words[v >> 5] >> (v & 31)) & ((1u << N) - 1u); }
+
+template <int N>
+__device__ __forceinline__ float sum_unnamed(const float* e, unsigned named) {
+  float s = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float e = __builtin_amdgcn_exp2f((x[u][i] - m0) * c);
-        st += e;
-        if (REST) rt += (named >> i & 1u) ? 0.0f : e;
+  for (int i = 0; i < N; ++i) s += (named >> i & 1u) ? 0.0f : e[i];
+  return s;
+}
+
+// A thread's share of a row that is streamed: its own running maximum, and sums that it rescales when a batch raises the maximum.
+template <bool REST>
+struct Running {
+  float m = -INFINITY, s = 0.0f, r = 0.0f;
+  __device__ __forceinline__ void raise(float to, float c) {
+    if (to > m) {
+      const float f = __builtin_amdgcn_exp2f((m - to) * c);
+      s *= f;
+      r *= f;
+      m = to;
+    }
+  }
+  // vectors [from, to) of z, G threads apart
+  template <typename T, int G>
+  __device__ __forceinline__ void stream(const T* z, int from, int to, float c, const unsigned* words, int tid) {
+    constexpr int U = 4, N = Vec16<T>::N;
+    for (int at = from + tid; at < to; at += U * G) {
+      u32x4 raw[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) raw[u] = at + u * G < to ? ldu<u32x4>(z + (size_t)(at + u * G) * N) : Vec16<T>::fill_minus_inf();
+      float bm = m;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float x[N];
+        Vec16<T>::unpack(raw[u], x);
+        bm = max_of<N>(x, bm);
+      }
+      raise(bm, c);
+      const Shift sh(m == -INFINITY ? 0.0f : m, c);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float x[N];
+        Vec16<T>::unpack(raw[u], x);
+        sh.exps<N>(x);
+        const float e = sum_of<N>(x);
+        s += e;
+        if constexpr (REST) {
+          const unsigned named = at + u * G < to ? named_bits<N>(words, (at + u * G) * N) : 0u;
+          r += named == 0u ? e : sum_unnamed<N>(x, named);
+        }
       }
     }
   }
-  m = group_reduce<MaxOp, G>(mt, red0);
-  const float f = __builtin_amdgcn_exp2f((mt - (m == -INFINITY ? 0.0f : m)) * c);
-  s = group_reduce<SumOp, G>(st * f, red1);
-  r = 0.0f;
-  if constexpr (REST) {                                      // red0 is free: every thread has read it before the barrier in the sum
-    r = group_reduce<SumOp, G>(rt * f, red0);
+  __device__ __forceinline__ void one(float x, float c, bool named) {
+    raise(x, c);
+    Shift(m == -INFINITY ? 0.0f : m, c).template exps<1>(&x);
+    s += x;
+    if (REST && !named) r += x;
   }
-}
+  // the sums with respect to a maximum over more threads; a thread that saw only -inf has sums of 0 (or NaN) and keeps them
+  __device__ __forceinline__ void about(float all, float c) {
+    if (m != -INFINITY) {
+      const float f = __builtin_amdgcn_exp2f((m - all) * c);
+      s *= f;
+      r *= f;
+    }
+  }
+};
 
-// What one wave makes of a row's teacher entries: p (into sp, 0 for padding), the tokens (into sid, -1 for padding), sum p and
-// sum p (log p - z / T).  FRL_DISTILL_REST needs 1 - sum p, which float32 exponentials would leave without digits: float64.
+// What one wave makes of a row's teacher entries: p (into sp, 0 for padding), the tokens (into sid, -1 for padding) and their logits
+// (into sz), sum p and sum p (log p - z / T).  FRL_DISTILL_REST needs 1 - sum p, which float32 exponentials would leave without digits: float64.
 template <typename T, bool REST>
-__device__ __forceinline__ void teacher_part(const DistillArgs& a, long long row, const T* z, int lane, int* sid, float* sp, double& sum_p, double& cross) {
+__device__ __forceinline__ void teacher_part(const DistillArgs& a, long long row, const T* z, int lane, int* sid, float* sp, float* sz, double& sum_p, double& cross) {
   sum_p = cross = 0.0;
   float tm = -INFINITY, tot = 0.0f;
   if constexpr (!REST) {
@@ -127,10 +178,11 @@ __device__ __forceinline__ void teacher_part(const DistillArgs& a, long long row
   for (int k = lane; k < a.top; k += 64) {
     const long long id = ld_id(a.ids, row * a.ids_stride + k, a.ids64);
     const bool valid = id >= 0 && id < a.vocab;
-    float p = 0.0f;
+    float p = 0.0f, zk = 0.0f;
     if (valid) {
       const float t = teacher_at(a.teacher, row * a.teacher_stride + k, a.teacher_dtype);
-      const float y = Elt<T>::get(z[id]) * a.inv_temp;
+      zk = Elt<T>::get(z[id]);
+      const float y = zk * a.inv_temp;
       float lp;
       if constexpr (REST) {
         const double pd = exp((double)t);
@@ -147,78 +199,99 @@ __device__ __forceinline__ void teacher_part(const DistillArgs& a, long long row
     }
     sid[k] = valid ? (int)id : -1;
     sp[k] = p;
+    sz[k] = zk;
   }
   sum_p = wave_reduce<SumOp>(sum_p);
   cross = wave_reduce<SumOp>(cross);
 }
 
-struct RowResult { float loss, inv_s, k_named, k_rest; };
+struct Factors { float inv_s, k_named, k_rest; };
 
 template <bool REST>
-__device__ __forceinline__ RowResult row_result(const DistillArgs& a, float m, float s, float r, double sum_p, double cross) {
-  RowResult o;
+__device__ __forceinline__ Factors row_factors(float s, float r, double sum_p) {
+  Factors o;
   o.inv_s = 1.0f / s;
-  double loss = cross + sum_p * ((double)m * (double)a.inv_temp + (double)logf(s));
   o.k_named = o.k_rest = (float)sum_p;
   if constexpr (REST) {
     const double P = 1.0 - sum_p;
     if (P > 0.0) {
-      loss += P * (log(P) - (double)(logf(r) - logf(s)));
       o.k_named = 1.0f;
       o.k_rest = 1.0f - (float)P * s / r;
     }
-  } else {
-    // softmax over the named entries sums to one; a row that names nothing has neither loss nor gradient
-    o.k_named = o.k_rest = sum_p != 0.0 ? 1.0f : 0.0f;
-    if (sum_p != sum_p) o.k_named = o.k_rest = (float)sum_p;
-    else if (sum_p == 0.0) loss = 0.0;
+  } else if (sum_p == sum_p) {
+    o.k_named = o.k_rest = sum_p != 0.0 ? 1.0f : 0.0f;     // a softmax sums to one; a row that names nothing has neither loss nor gradient
   }
-  o.loss = (float)loss;
   return o;
+}
+
+template <bool REST>
+__device__ __forceinline__ float row_loss(const DistillArgs& a, float m, float s, float r, double sum_p, double cross) {
+  if (!REST && sum_p == 0.0) return 0.0f;
+  double loss = cross + sum_p * ((double)m * (double)a.inv_temp + log((double)s));
+  if constexpr (REST) {
+    const double P = 1.0 - sum_p;
+    if (P > 0.0) loss += P * log(P * (double)s / (double)r);
+  }
+  return (float)loss;
 }
 
 template <typename T, int G>
 __device__ __forceinline__ void zero_row(T* g, int n, int tid) {
-  for (int v = 4 * tid; v < n; v += 4 * G) {
-    if (n - v >= 4) Elt<T>::store4(g + v, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
-    else for (int i = 0; i < n - v; ++i) g[v + i] = Elt<T>::put(0.0f);
+  constexpr int N = Vec16<T>::N;
+  const int nvec = n / N, tail = n - nvec * N;
+  for (int at = tid; at < nvec; at += G) stu(g + (size_t)at * N, u32x4{0u, 0u, 0u, 0u});
+  if (tid < tail) g[nvec * N + tid] = Elt<T>::put(0.0f);
+}
+
+// f_rest 2^((x - m) c) of a vector.  A two-byte gradient takes |f_rest| into the exponent while |M| < 128 rounds M - log2 |f_rest| by less than 2^-17
+// (the gradient's own rounding is 2^-11 or 2^-8).
+template <typename T>
+struct Scaled {
+  Shift sh;
+  float f, M;
+  unsigned sign;
+  __device__ __forceinline__ Scaled(const Shift& s, float f_rest) : sh(s), f(f_rest), M(s.M - __builtin_amdgcn_logf(fabsf(f_rest))), sign(f_rest < 0.0f ? 0x80008000u : 0u) {}
+  __device__ __forceinline__ u32x4 of(u32x4 raw) const {
+    constexpr int N = Vec16<T>::N;
+    float x[N];
+    Vec16<T>::unpack(raw, x);
+    if (sizeof(T) == 2 && fabsf(sh.M) < 128.0f) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], sh.c, -M));
+      u32x4 r = Vec16<T>::pack(x);
+      r ^= sign;
+      return r;
+    }
+    sh.exps<N>(x);
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] *= f;
+    return Vec16<T>::pack(x);
+  }
+  __device__ __forceinline__ float one(float x) const {
+    sh.exps<1>(&x);
+    return f * x;
+  }
+};
+
+template <typename T, int G>
+__device__ __forceinline__ void stream_gradient(const T* z, T* g, int from, int to, const Scaled<T>& sc, int tid) {
+  constexpr int U = 4, N = Vec16<T>::N;
+  for (int at = from + tid; at < to; at += U * G) {
+    u32x4 raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (at + u * G < to) raw[u] = ldu<u32x4>(z + (size_t)(at + u * G) * N);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (at + u * G < to) stu(g + (size_t)(at + u * G) * N, sc.of(raw[u]));
   }
 }
 
-// Gradient of entries [v0, v0 + n): the scaled exponential everywhere, then the named entries over it.  Both are plain stores of one
-// workgroup with a barrier between them, so the second is what stays.
+// The named entries of [v0, v0 + n), over what the scaled exponentials put there.  Both are plain stores of one workgroup with a barrier
+// between them, so these are what stays; of a token named twice the first entry writes, with both probabilities.
 template <typename T, int G>
-__device__ __forceinline__ void row_gradient(const DistillArgs& a, const T* z, T* g, int v0, int n, float m, float inv_s, float k_named, float k_rest,
-                                             float f, const int* sid, const float* sp, int tid) {
-  constexpr int U = 4;
-  if (k_named == 0.0f && k_rest == 0.0f) {                   // the row names nothing: no gradient, whatever stands in the logits
-    zero_row<T, G>(g + v0, n, tid);
-    return;
-  }
-  const float c = a.scale2, f_rest = f * k_rest * inv_s, f_named = f * k_named * inv_s;
-  for (int v = 4 * tid; v < n; v += 4 * U * G) {
-    f32x4 x[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int at = v + 4 * G * u;
-      x[u] = quad(z + v0 + at, n - at);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int at = v + 4 * G * u, left = n - at;
-      f32x4 o;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = f_rest * __builtin_amdgcn_exp2f((x[u][i] - m) * c);
-      T* to = g + v0 + at;
-      if (left >= 4) Elt<T>::store4(to, o);
-      else {
-        if (left > 0) to[0] = Elt<T>::put(o[0]);
-        if (left > 1) to[1] = Elt<T>::put(o[1]);
-        if (left > 2) to[2] = Elt<T>::put(o[2]);
-      }
-    }
-  }
-  group_sync<G>();
+__device__ __forceinline__ void named_gradient(const DistillArgs& a, T* g, int v0, int n, const Shift& sh, float f_named, float f, const int* sid, const float* sp,
+                                               const float* sz, int tid) {
   for (int k = tid; k < a.top; k += G) {
     const int id = sid[k];
     if (id < v0 || id >= v0 + n) continue;
@@ -226,51 +299,129 @@ __device__ __forceinline__ void row_gradient(const DistillArgs& a, const T* z, T
     bool first = true;
     for (int j = 0; j < a.top; ++j)
       if (sid[j] == id) { p += sp[j]; first = first && j >= k; }
-    if (first) g[id] = Elt<T>::put(f_named * __builtin_amdgcn_exp2f((Elt<T>::get(z[id]) - m) * c) - f * p);
+    if (!first) continue;
+    float x = sz[k];
+    sh.exps<1>(&x);
+    g[id] = Elt<T>::put(f_named * x - f * p);
   }
 }
 
-// A row to a group: value, what the backward needs, and (GRAD) the gradient.
-template <typename T, int G, bool REST, bool GRAD>
-__global__ void __launch_bounds__(G == 64 ? 256 : G) frl_distill_row_kernel(const DistillArgs a) {
+// Between two passes over the vectors: the compiler may not carry their unpacked elements from one to the other, twice the registers.
+template <int NV>
+__device__ __forceinline__ void keep_packed(u32x4* raw) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(raw[i]));
+}
+
+// The thread's number as a value of its own: what is derived from it, an index and an address per vector, is then computed where it is used and not
+// kept in registers across the passes and rows.
+__device__ __forceinline__ int fresh(int tid) {
+  asm volatile("" : "+v"(tid));
+  return tid;
+}
+
+// A row to a group, its first NV vectors per thread held in registers: value, what the backward needs, and (GRAD) the gradient.
+template <typename T, int G, int NV, bool REST, bool GRAD>
+__global__ void __launch_bounds__(G == 64 ? 256 : G, 4) frl_distill_row_kernel(const DistillArgs a) {
   extern __shared__ __align__(16) unsigned lds[];
-  constexpr int GPB = G == 64 ? 4 : 1;
+  constexpr int GPB = G == 64 ? 4 : 1, N = Vec16<T>::N;
   __shared__ float red0[G / 64], red1[G / 64];
   __shared__ double row_p[GPB], row_x[GPB];
-  const int tid = threadIdx.x % G, grp = threadIdx.x / G;
+  const int tid = threadIdx.x % G, grp = G == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
   const int nwords = REST ? (a.vocab + 31) / 32 : 0;
-  unsigned* words = lds + (size_t)grp * (nwords + 2 * a.top);
+  unsigned* words = lds + (size_t)grp * (nwords + 3 * a.top);
   int* sid = (int*)(words + nwords);
   float* sp = (float*)(sid + a.top);
+  float* sz = sp + a.top;
   const float inv = a.inv_denom != nullptr ? *a.inv_denom : a.denom_scale;
-  for (long long row = (long long)blockIdx.x * GPB + grp; row < a.rows; row += (long long)gridDim.x * GPB) {
-    const T* z = (const T*)a.logits + row * a.logits_stride;
-    T* g = GRAD ? (T*)a.grad + row * a.grad_stride : nullptr;
-    const float w = a.weights != nullptr ? a.weights[row] : 1.0f;
-    if (w == 0.0f) {                                       // uniform over the group
-      if (tid == 0) {
-        a.rowloss[row] = 0.0f;
-        if (a.stats != nullptr) *(f32x4*)(a.stats + 4 * row) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      }
-      if constexpr (GRAD) zero_row<T, G>(g, a.vocab, tid);
-      continue;
-    }
-    if constexpr (REST) mark_named<G>(a, row, tid, 0, a.vocab, words);
-    if (tid < 64) {
-      double sum_p, cross;
-      teacher_part<T, REST>(a, row, z, tid, sid, sp, sum_p, cross);
-      if (tid == 0) { row_p[grp] = sum_p; row_x[grp] = cross; }
-    }
-    float m, s, r;
-    row_sums<T, G, REST>(z, a.vocab, a.scale2, words, tid, red0, red1, m, s, r);
-    group_sync<G>();                                       // the teacher's part is visible (and red1 free)
-    const RowResult o = row_result<REST>(a, m, s, r, row_p[grp], row_x[grp]);
+  const int nvec = a.vocab / N, tail = a.vocab - nvec * N, nv = (nvec + G - 1) / G;
+  const long long row = block_index() * GPB + grp;
+  if (row >= a.rows) return;
+  const T* z = (const T*)a.logits + row * a.logits_stride;
+  T* g = GRAD ? (T*)a.grad + row * a.grad_stride : nullptr;
+  const float w = a.weights != nullptr ? a.weights[row] : 1.0f;
+  if (w == 0.0f) {                                       // uniform over the group
     if (tid == 0) {
-      a.rowloss[row] = w * o.loss;
-      if (a.stats != nullptr) *(f32x4*)(a.stats + 4 * row) = f32x4{m, o.inv_s, o.k_named, o.k_rest};
+      a.rowloss[row] = 0.0f;
+      if (a.stats != nullptr) *(f32x4*)(a.stats + 4 * row) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    if constexpr (GRAD) row_gradient<T, G>(a, z, g, 0, a.vocab, m, o.inv_s, o.k_named, o.k_rest, w * inv * a.inv_temp, sid, sp, tid);
-    group_sync<G>();                                       // the next row writes the shared arrays again
+    if constexpr (GRAD) zero_row<T, G>(g, a.vocab, tid);
+    return;
+  }
+  // the teacher's part first: its float64 temporaries and the row's vectors together would not fit 128 registers
+  if constexpr (REST) mark_named<G>(a, row, tid, 0, a.vocab, words);
+  if (tid < 64) {
+    double sum_p, cross;
+    teacher_part<T, REST>(a, row, z, tid, sid, sp, sz, sum_p, cross);
+    if (tid == 0) { row_p[grp] = sum_p; row_x[grp] = cross; }
+  }
+  constexpr int R = NV > 0 ? NV : 1;
+  u32x4 raw[R];
+  const int t0 = fresh(tid);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    raw[i] = Vec16<T>::fill_minus_inf();
+    if (i < nv && i * G + t0 < nvec) raw[i] = ldu<u32x4>((const char*)z + 16u * (unsigned)(i * G + t0));
+  }
+  Running<REST> run;
+  if (nvec > NV * G) run.template stream<T, G>(z, NV * G, nvec, a.scale2, words, t0);
+  if (tid < tail) run.one(Elt<T>::get(z[nvec * N + tid]), a.scale2, REST && named_bits<1>(words, nvec * N + tid) != 0u);
+  float m = run.m;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (i < nv) {
+      float x[N];
+      Vec16<T>::unpack(raw[i], x);
+      m = max_of<N>(x, m);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  m = group_reduce<MaxOp, G>(m, red0);
+  run.about(m, a.scale2);
+  const Shift sh(m, a.scale2);
+  keep_packed<NV>(raw);
+  const int t1 = fresh(tid);
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (i < nv) {
+      float x[N];
+      Vec16<T>::unpack(raw[i], x);
+      sh.exps<N>(x);
+      const float e = sum_of<N>(x);
+      run.s += e;
+      if constexpr (REST) {
+        const unsigned named = i * G + t1 < nvec ? named_bits<N>(words, (i * G + t1) * N) : 0u;
+        run.r += named == 0u ? e : sum_unnamed<N>(x, named);
+      }
+      __builtin_amdgcn_sched_barrier(0);                     // one vector unpacked at a time: eight independent elements are parallel enough
+    }
+  const float s = group_reduce<SumOp, G>(run.s, red1);
+  const float r = REST ? group_reduce<SumOp, G>(run.r, red0) : 0.0f;   // red0: every thread has read the maximum before the barrier in the sum
+  if constexpr (G == 64) group_sync<G>();                    // the teacher's part is visible (a workgroup has passed barriers since)
+  const double sum_p = row_p[grp];
+  const Factors k = row_factors<REST>(s, r, sum_p);
+  if constexpr (GRAD) {
+    const float f = w * inv * a.inv_temp;
+    if (k.k_named == 0.0f && k.k_rest == 0.0f) {
+      zero_row<T, G>(g, a.vocab, tid);
+    } else {
+      const Scaled<T> sc(sh, f * k.k_rest * k.inv_s);
+      keep_packed<NV>(raw);
+      const int t2 = fresh(tid);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (i < nv && i * G + t2 < nvec) {
+          stu((char*)g + 16u * (unsigned)(i * G + t2), sc.of(raw[i]));
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      if (nvec > NV * G) stream_gradient<T, G>(z, g, NV * G, nvec, sc, t2);
+      if (tid < tail) g[nvec * N + tid] = Elt<T>::put(sc.one(Elt<T>::get(z[nvec * N + tid])));
+      group_sync<G>();
+      named_gradient<T, G>(a, g, 0, a.vocab, sh, f * k.k_named * k.inv_s, f, sid, sp, sz, tid);
+    }
+  }
+  if (tid == 0) {
+    a.rowloss[row] = w * row_loss<REST>(a, m, s, r, sum_p, row_x[grp]);
+    if (a.stats != nullptr) *(f32x4*)(a.stats + 4 * row) = f32x4{m, k.inv_s, k.k_named, k.k_rest};
   }
 }
 
@@ -280,14 +431,23 @@ template <typename T, int G, bool REST>
 __global__ void __launch_bounds__(G) frl_distill_part_kernel(const DistillArgs a) {
   extern __shared__ __align__(16) unsigned lds[];
   __shared__ float red0[G / 64], red1[G / 64];
-  const long long row = blockIdx.x / a.segs;
-  const int seg = blockIdx.x % a.segs, v0 = seg * a.seg_len, n = min(a.vocab - v0, a.seg_len);
+  const long long item = block_index();
+  if (item >= a.rows * a.segs) return;
+  const long long row = item / a.segs;
+  const int v0 = (int)(item - row * a.segs) * a.seg_len, n = min(a.vocab - v0, a.seg_len);
   if (a.weights != nullptr && a.weights[row] == 0.0f) return;
   if constexpr (REST) mark_named<G>(a, row, threadIdx.x, v0, n, lds);
-  float m, s, r;
-  row_sums<T, G, REST>((const T*)a.logits + row * a.logits_stride + v0, n, a.scale2, lds, threadIdx.x, red0, red1, m, s, r);
+  const T* z = (const T*)a.logits + row * a.logits_stride + v0;
+  constexpr int N = Vec16<T>::N;
+  const int nvec = n / N, tid = threadIdx.x;
+  Running<REST> run;
+  run.template stream<T, G>(z, 0, nvec, a.scale2, lds, tid);
+  if (tid < n - nvec * N) run.one(Elt<T>::get(z[nvec * N + tid]), a.scale2, REST && named_bits<1>(lds, nvec * N + tid) != 0u);
+  const float m = group_reduce<MaxOp, G>(run.m, red0);
+  run.about(m, a.scale2);
+  const float s = group_reduce<SumOp, G>(run.s, red1), r = REST ? group_reduce<SumOp, G>(run.r, red0) : 0.0f;   // red0: read before the barrier in the sum
   if (threadIdx.x == 0) {
-    float* p = a.part + 3 * (row * a.segs + seg);
+    float* p = a.part + 3 * item;
     p[0] = m; p[1] = s; p[2] = r;
   }
 }
@@ -298,8 +458,10 @@ __global__ void __launch_bounds__(64) frl_distill_join_kernel(const DistillArgs 
   extern __shared__ __align__(16) unsigned lds[];
   int* sid = (int*)lds;
   float* sp = (float*)(sid + a.top);
-  const long long row = blockIdx.x;
+  float* sz = sp + a.top;
   const int lane = threadIdx.x;
+  const long long row = block_index();
+  if (row >= a.rows) return;
   const float w = a.weights != nullptr ? a.weights[row] : 1.0f;
   if (w == 0.0f) {
     if (lane == 0) {
@@ -309,23 +471,22 @@ __global__ void __launch_bounds__(64) frl_distill_join_kernel(const DistillArgs 
     return;
   }
   double sum_p, cross;
-  teacher_part<T, REST>(a, row, (const T*)a.logits + row * a.logits_stride, lane, sid, sp, sum_p, cross);
+  teacher_part<T, REST>(a, row, (const T*)a.logits + row * a.logits_stride, lane, sid, sp, sz, sum_p, cross);
   float m = -INFINITY, s = 0.0f, r = 0.0f;
   const float* p = a.part + 3 * row * a.segs;
   for (int i = lane; i < a.segs; i += 64) m = fmaxf(m, p[3 * i]);
   m = wave_reduce<MaxOp>(m);
-  const float m0 = m == -INFINITY ? 0.0f : m;
   for (int i = lane; i < a.segs; i += 64) {
-    const float f = __builtin_amdgcn_exp2f((p[3 * i] - m0) * a.scale2);
+    const float f = p[3 * i] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((p[3 * i] - m) * a.scale2);     // a segment of -inf alone has sums of 0 (or NaN)
     s += p[3 * i + 1] * f;
     r += p[3 * i + 2] * f;
   }
   s = wave_reduce<SumOp>(s);
   r = wave_reduce<SumOp>(r);
-  const RowResult o = row_result<REST>(a, m, s, r, sum_p, cross);
+  const Factors k = row_factors<REST>(s, r, sum_p);
   if (lane == 0) {
-    a.rowloss[row] = w * o.loss;
-    if (a.stats != nullptr) *(f32x4*)(a.stats + 4 * row) = f32x4{m, o.inv_s, o.k_named, o.k_rest};
+    a.rowloss[row] = w * row_loss<REST>(a, m, s, r, sum_p, cross);
+    if (a.stats != nullptr) *(f32x4*)(a.stats + 4 * row) = f32x4{m, k.inv_s, k.k_named, k.k_rest};
   }
 }
 
@@ -333,32 +494,37 @@ __global__ void __launch_bounds__(64) frl_distill_join_kernel(const DistillArgs 
 template <typename T, int G, bool REST>
 __global__ void __launch_bounds__(G == 64 ? 256 : G) frl_distill_grad_kernel(const DistillArgs a) {
   extern __shared__ __align__(16) unsigned lds[];
-  constexpr int GPB = G == 64 ? 4 : 1;
-  const int tid = threadIdx.x % G, grp = threadIdx.x / G;
-  int* sid = (int*)lds + (size_t)grp * 2 * a.top;
+  constexpr int GPB = G == 64 ? 4 : 1, N = Vec16<T>::N;
+  const int tid = threadIdx.x % G, grp = G == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+  int* sid = (int*)lds + (size_t)grp * 3 * a.top;
   float* sp = (float*)(sid + a.top);
+  float* sz = sp + a.top;
   const float inv = a.inv_denom != nullptr ? *a.inv_denom : a.denom_scale;
-  const long long items = a.rows * a.segs;
-  for (long long item = (long long)blockIdx.x * GPB + grp; item < items; item += (long long)gridDim.x * GPB) {
-    const long long row = item / a.segs;
-    const int v0 = (int)(item - row * a.segs) * a.seg_len, n = min(a.vocab - v0, a.seg_len);
-    const T* z = (const T*)a.logits + row * a.logits_stride;
-    T* g = (T*)a.grad + row * a.grad_stride;
-    const float w = a.weights != nullptr ? a.weights[row] : 1.0f;
-    if (w == 0.0f) {
-      zero_row<T, G>(g + v0, n, tid);
-      continue;
-    }
-    if (tid < 64) {
-      double sum_p, cross;
-      teacher_part<T, REST>(a, row, z, tid, sid, sp, sum_p, cross);
-    }
-    const f32x4 st = *(const f32x4*)(a.stats + 4 * row);
-    const float cot = a.g_loss != nullptr ? a.g_loss[row * a.g_stride] : 1.0f;
-    group_sync<G>();
-    row_gradient<T, G>(a, z, g, v0, n, st[0], st[1], st[2], st[3], cot * w * inv * a.inv_temp, sid, sp, tid);
-    group_sync<G>();
+  const long long item = block_index() * GPB + grp;
+  if (item >= a.rows * a.segs) return;
+  const long long row = item / a.segs;
+  const int v0 = (int)(item - row * a.segs) * a.seg_len, n = min(a.vocab - v0, a.seg_len);
+  const T* z = (const T*)a.logits + row * a.logits_stride;
+  T* g = (T*)a.grad + row * a.grad_stride;
+  const float w = a.weights != nullptr ? a.weights[row] : 1.0f;
+  const f32x4 st = *(const f32x4*)(a.stats + 4 * row);
+  if (w == 0.0f || (st[2] == 0.0f && st[3] == 0.0f)) {
+    zero_row<T, G>(g + v0, n, tid);
+    return;
   }
+  const float cot = a.g_loss != nullptr ? a.g_loss[row * a.g_stride] : 1.0f;
+  const float f = cot * w * inv * a.inv_temp;
+  const Shift sh(st[0], a.scale2);
+  const Scaled<T> sc(sh, f * st[3] * st[1]);
+  const int nvec = n / N, tail = n - nvec * N;
+  stream_gradient<T, G>(z + v0, g + v0, 0, nvec, sc, tid);
+  if (tid < tail) g[v0 + nvec * N + tid] = Elt<T>::put(sc.one(Elt<T>::get(z[v0 + nvec * N + tid])));
+  if (tid < 64) {
+    double sum_p, cross;
+    teacher_part<T, REST>(a, row, z, tid, sid, sp, sz, sum_p, cross);
+  }
+  group_sync<G>();
+  named_gradient<T, G>(a, g, v0, n, sh, f * st[2] * st[1], f, sid, sp, sz, tid);
 }
 
 // ---- over the rows ------------------------------------------------------------------------------------------------------
@@ -393,23 +559,34 @@ __global__ void __launch_bounds__(1024) frl_distill_sum_kernel(const float* __re
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
 
-struct DistillPlan { int G, segs, seg_len; };
+struct DistillPlan { int G, NV, segs, seg_len; bool split; };
 
-static DistillPlan distill_plan(long long rows, int vocab) {
-  DistillPlan p;
-  p.G = vocab <= 1024 ? 64 : vocab <= 8192 ? 256 : 1024;
-  p.segs = 1;
-  p.seg_len = vocab;
-  if (p.G == 1024 && rows > 0 && (rows < 256 || vocab > DSEG_MAX)) {
-    // enough segments for two workgroups per CU, of at least 4096 entries
-    long long want = (512 + rows - 1) / rows;
-    const long long most = (vocab + 4095) / 4096, least = ((long long)vocab + DSEG_MAX - 1) / DSEG_MAX;
-    if (want > most) want = most;
-    if (want < least) want = least;
-    p.seg_len = (int)(((vocab + want - 1) / want + 31) / 32 * 32);
-    p.segs = (vocab + p.seg_len - 1) / p.seg_len;
-    if (p.segs > 1) p.G = 256;
+// Threads per row: as few as hold it with 16 vectors of 16 bytes each, more while the rows alone leave the chip's 1024 SIMDs short of four
+// waves.  A value alone keeps nothing and streams, up to 1024 threads; a gradient keeps what 512 threads hold (two workgroups to a CU, one
+// loads while the other computes) and reads the rest of a longer row again.  Measured, bf16, value + gradient: 8192 x 131072 990 us so, 1127
+// with 1024 threads and all of it held, 1158 with nothing held; 4096 x 32000 130 with 256 threads, 157 with 512; 2048 x 131072, value alone:
+// 95 us streamed by 1024 threads, 115 held by 512.
+// Fewer than 256 rows of more than 8192 entries, and rows whose named bits would take more than 32 KB of LDS, are split: at least 512 segments,
+// each of 4096 to 65536 entries.
+static DistillPlan distill_plan(long long rows, int vocab, int dtype, bool grad) {
+  const int vec = dtype == FRL_ELT_F32 ? 4 : 8;
+  DistillPlan p = {64, 0, 1, vocab, false};
+  if (vocab <= DROW_MAX && !(rows < 256 && vocab > 8192)) {
+    const int most = grad ? 512 : 1024;
+    auto next = [](int G) { return G == 64 ? 256 : 2 * G; };
+    while (p.G < most && vocab > p.G * 16 * vec) p.G = next(p.G);
+    while (p.G < most && rows * p.G < 4096 * 64 && vocab > 2 * p.G * vec) p.G = next(p.G);
+    if (grad) p.NV = vocab <= p.G * 4 * vec ? 4 : 16;
+    return p;
   }
+  p.G = 256;
+  long long want = rows > 0 ? (512 + rows - 1) / rows : 1;
+  const long long most = ((long long)vocab + 4095) / 4096, least = ((long long)vocab + DSEG_MAX - 1) / DSEG_MAX;
+  if (want > most) want = most;
+  if (want < least) want = least;
+  p.seg_len = (int)(((vocab + want - 1) / want + 31) / 32 * 32);
+  p.segs = (vocab + p.seg_len - 1) / p.seg_len;
+  p.split = true;
   return p;
 }
 
@@ -425,8 +602,6 @@ static int distill_validate(const FrlDistillDesc* d) {
   if (d->top > FRL_DISTILL_MAX_TOP) { set_error("distill: top %d > %d", d->top, FRL_DISTILL_MAX_TOP); return FRL_EUNSUPPORTED; }
   if (d->vocab > (1 << 30)) { set_error("distill: vocab %d > 2^30", d->vocab); return FRL_EUNSUPPORTED; }
   if (d->rows > (1LL << 30)) { set_error("distill: %lld rows > 2^30", (long long)d->rows); return FRL_EUNSUPPORTED; }
-  const DistillPlan p = distill_plan(d->rows, d->vocab);
-  if (p.segs > 1 && d->rows * p.segs > (1LL << 22)) { set_error("distill: %lld rows of %d entries are more than 2^22 segments in one call", (long long)d->rows, d->vocab); return FRL_EUNSUPPORTED; }
   if (d->rows > 1 && d->logits_stride < d->vocab) { set_error("distill: row stride %lld < vocab %d", (long long)d->logits_stride, d->vocab); return FRL_EINVAL; }
   return FRL_OK;
 }
@@ -459,45 +634,56 @@ static DistillWs distill_ws(const FrlDistillDesc* d, const DistillPlan& p) {
   w.inv = up((size_t)d->rows);
   w.stats = w.inv + 64;
   w.part = w.stats + up(4 * (size_t)(d->rows + 1));
-  w.total = (w.part + (p.segs > 1 ? up(3 * (size_t)d->rows * p.segs) : 0)) * sizeof(float);
+  w.total = (w.part + (p.split ? up(3 * (size_t)d->rows * p.segs) : 0)) * sizeof(float);
   return w;
 }
 
 template <typename T, bool REST>
-static hipError_t launch_rows(const DistillArgs& a, int G, bool grad, hipStream_t st) {
-  const size_t per = ((size_t)(REST ? (a.vocab + 31) / 32 : 0) + 2 * (size_t)a.top) * 4;
-  const size_t lds = G == 64 ? 4 * per : per;
-  const long long blocks = G == 64 ? (a.rows + 3) / 4 : a.rows;
-  const unsigned grid = (unsigned)(blocks < (1 << 20) ? blocks : (1 << 20));
-#define FRL_GO(g, gr) hipLaunchKernelGGL((frl_distill_row_kernel<T, g, REST, gr>), dim3(grid), dim3(g == 64 ? 256 : g), lds, st, a)
-  if (G == 64) { if (grad) FRL_GO(64, true); else FRL_GO(64, false); }
-  else if (G == 256) { if (grad) FRL_GO(256, true); else FRL_GO(256, false); }
-  else { if (grad) FRL_GO(1024, true); else FRL_GO(1024, false); }
+static hipError_t launch_rows(const DistillArgs& a, const DistillPlan& p, bool grad, hipStream_t st) {
+  const size_t per = ((size_t)(REST ? (a.vocab + 31) / 32 : 0) + 3 * (size_t)a.top) * 4;
+  const size_t lds = p.G == 64 ? 4 * per : per;
+  const long long blocks = p.G == 64 ? (a.rows + 3) / 4 : a.rows;
+  const dim3 grid = grid_of(blocks);
+#define FRL_GO(g, nv, gr) hipLaunchKernelGGL((frl_distill_row_kernel<T, g, nv, REST, gr>), grid, dim3(g == 64 ? 256 : g), lds, st, a)
+  if (!grad) {
+    if (p.G == 64) FRL_GO(64, 0, false);
+    else if (p.G == 256) FRL_GO(256, 0, false);
+    else if (p.G == 512) FRL_GO(512, 0, false);
+    else FRL_GO(1024, 0, false);
+  } else if (p.NV == 4) {
+    if (p.G == 64) FRL_GO(64, 4, true);
+    else if (p.G == 256) FRL_GO(256, 4, true);
+    else FRL_GO(512, 4, true);
+  } else {
+    if (p.G == 64) FRL_GO(64, 16, true);
+    else if (p.G == 256) FRL_GO(256, 16, true);
+    else FRL_GO(512, 16, true);
+  }
 #undef FRL_GO
-  note_kernel("frl_distill_row_kernel<%s, %d threads> [%u]", grad ? "value + gradient" : "value", G, grid);
+  note_kernel("frl_distill_row_kernel<%s, %d threads, %d vectors> [%lld]", grad ? "value + gradient" : "value", p.G, p.NV, blocks);
   return hipGetLastError();
 }
 
 template <typename T, bool REST>
 static hipError_t launch_parts(const DistillArgs& a, hipStream_t st) {
-  const unsigned grid = (unsigned)(a.rows * a.segs);
-  hipLaunchKernelGGL((frl_distill_part_kernel<T, 256, REST>), dim3(grid), dim3(256), REST ? (size_t)(a.seg_len / 32) * 4 : 0, st, a);
+  const long long items = a.rows * a.segs;
+  hipLaunchKernelGGL((frl_distill_part_kernel<T, 256, REST>), grid_of(items), dim3(256), REST ? (size_t)((a.seg_len + 31) / 32) * 4 : 0, st, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((frl_distill_join_kernel<T, REST>), dim3((unsigned)a.rows), dim3(64), (size_t)a.top * 8, st, a);
-  note_kernel("frl_distill_part_kernel [%u] + frl_distill_join_kernel [%lld]", grid, a.rows);
+  hipLaunchKernelGGL((frl_distill_join_kernel<T, REST>), grid_of(a.rows), dim3(64), (size_t)a.top * 12, st, a);
+  note_kernel("frl_distill_part_kernel [%lld] + frl_distill_join_kernel [%lld]", items, a.rows);
   return hipGetLastError();
 }
 
 template <typename T, bool REST>
-static hipError_t launch_grad(const DistillArgs& a, int G, hipStream_t st) {
-  const long long items = a.rows * a.segs, blocks = G == 64 ? (items + 3) / 4 : items;
-  const unsigned grid = (unsigned)(blocks < (1 << 20) ? blocks : (1 << 20));
-  const size_t lds = (size_t)a.top * 8 * (G == 64 ? 4 : 1);
-  if (G == 64) hipLaunchKernelGGL((frl_distill_grad_kernel<T, 64, REST>), dim3(grid), dim3(256), lds, st, a);
-  else if (G == 256) hipLaunchKernelGGL((frl_distill_grad_kernel<T, 256, REST>), dim3(grid), dim3(256), lds, st, a);
-  else hipLaunchKernelGGL((frl_distill_grad_kernel<T, 1024, REST>), dim3(grid), dim3(1024), lds, st, a);
-  note_kernel("frl_distill_grad_kernel<%d threads> [%u]", G, grid);
+static hipError_t launch_grad(const DistillArgs& a, const DistillPlan& p, hipStream_t st) {
+  const long long items = a.rows * a.segs, blocks = p.G == 64 ? (items + 3) / 4 : items;
+  const dim3 grid = grid_of(blocks);
+  const size_t lds = (size_t)a.top * 12 * (p.G == 64 ? 4 : 1);
+  if (p.G == 64) hipLaunchKernelGGL((frl_distill_grad_kernel<T, 64, REST>), grid, dim3(256), lds, st, a);
+  else if (p.G == 256) hipLaunchKernelGGL((frl_distill_grad_kernel<T, 256, REST>), grid, dim3(256), lds, st, a);
+  else hipLaunchKernelGGL((frl_distill_grad_kernel<T, 1024, REST>), grid, dim3(1024), lds, st, a);
+  note_kernel("frl_distill_grad_kernel<%d threads> [%lld]", p.G, blocks);
   return hipGetLastError();
 }
 
@@ -513,7 +699,7 @@ extern "C" {
 
 size_t frl_distill_workspace_bytes(const FrlDistillDesc* desc) {
   if (distill_validate(desc) != FRL_OK) return 0;
-  return distill_ws(desc, distill_plan(desc->rows, desc->vocab)).total;
+  return distill_ws(desc, distill_plan(desc->rows, desc->vocab, desc->dtype, true)).total;
 }
 
 int frl_distill_fwd(const FrlDistillDesc* desc, const FrlDistillBufs* bufs, void* workspace, size_t workspace_bytes, void* hip_stream) {
@@ -527,7 +713,7 @@ int frl_distill_fwd(const FrlDistillDesc* desc, const FrlDistillBufs* bufs, void
   const bool grad = bufs->grad != nullptr && desc->rows > 0;
   if (grad && desc->rows > 1 && desc->grad_stride < desc->vocab) { set_error("distill: grad row stride %lld < vocab %d", (long long)desc->grad_stride, desc->vocab); return FRL_EINVAL; }
   if (grad && distill_overlap(desc, bufs)) { set_error("distill: grad overlaps logits"); return FRL_EINVAL; }
-  const DistillPlan p = distill_plan(desc->rows, desc->vocab);
+  const DistillPlan p = distill_plan(desc->rows, desc->vocab, desc->dtype, grad);
   const DistillWs w = distill_ws(desc, p);
   if (workspace == nullptr || ((uintptr_t)workspace & 255) != 0) { set_error("workspace must be non-NULL and 256-byte aligned"); return FRL_EWORKSPACE; }
   if (workspace_bytes < w.total) { set_error("workspace %zu B < required %zu B", workspace_bytes, w.total); return FRL_EWORKSPACE; }
@@ -535,7 +721,7 @@ int frl_distill_fwd(const FrlDistillDesc* desc, const FrlDistillBufs* bufs, void
   hipStream_t st = (hipStream_t)hip_stream;
   DistillArgs a = distill_args(desc, bufs, p);
   const int dtype = desc->dtype;
-  const bool rest = desc->kind == FRL_DISTILL_REST, split = p.segs > 1;
+  const bool rest = desc->kind == FRL_DISTILL_REST, split = p.split;
   a.rowloss = desc->reduction == FRL_REDUCE_NONE ? bufs->loss : ws + w.rowloss;
   a.stats = bufs->row_stats != nullptr ? bufs->row_stats : (split && grad) ? ws + w.stats : nullptr;
   a.part = ws + w.part;
@@ -550,9 +736,9 @@ int frl_distill_fwd(const FrlDistillDesc* desc, const FrlDistillBufs* bufs, void
   if (e == hipSuccess && desc->rows > 0) {
     if (split) {
       e = FRL_BY_TYPE(launch_parts)(a, st);
-      if (e == hipSuccess && grad) e = FRL_BY_TYPE(launch_grad)(a, p.G, st);
+      if (e == hipSuccess && grad) e = FRL_BY_TYPE(launch_grad)(a, p, st);
     } else {
-      e = FRL_BY_TYPE(launch_rows)(a, p.G, grad, st);
+      e = FRL_BY_TYPE(launch_rows)(a, p, grad, st);
     }
   }
   if (e == hipSuccess && desc->reduction != FRL_REDUCE_NONE) {
@@ -574,7 +760,7 @@ int frl_distill_bwd(const FrlDistillDesc* desc, const FrlDistillBufs* bufs, void
   if (((uintptr_t)bufs->row_stats & 15) != 0) { set_error("distill: bufs.row_stats must be 16-byte aligned"); return FRL_EINVAL; }
   if (desc->rows > 1 && desc->grad_stride < desc->vocab) { set_error("distill: grad row stride %lld < vocab %d", (long long)desc->grad_stride, desc->vocab); return FRL_EINVAL; }
   if (distill_overlap(desc, bufs)) { set_error("distill: grad overlaps logits"); return FRL_EINVAL; }
-  const DistillPlan p = distill_plan(desc->rows, desc->vocab);
+  const DistillPlan p = distill_plan(desc->rows, desc->vocab, desc->dtype, false);
   DistillArgs a = distill_args(desc, bufs, p);
   a.stats = bufs->row_stats;
   a.g_loss = bufs->g_loss;
@@ -582,7 +768,7 @@ int frl_distill_bwd(const FrlDistillDesc* desc, const FrlDistillBufs* bufs, void
   if (desc->reduction == FRL_REDUCE_MEAN && bufs->weights != nullptr) a.inv_denom = bufs->row_stats + 4 * desc->rows;
   const int dtype = desc->dtype;
   const bool rest = desc->kind == FRL_DISTILL_REST;
-  const hipError_t e = FRL_BY_TYPE(launch_grad)(a, p.G, (hipStream_t)hip_stream);
+  const hipError_t e = FRL_BY_TYPE(launch_grad)(a, p, (hipStream_t)hip_stream);
   if (e != hipSuccess) { set_error("distill gradient launch: %s", hipGetErrorString(e)); return FRL_EHIP; }
   return FRL_OK;
 }

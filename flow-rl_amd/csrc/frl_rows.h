@@ -56,6 +56,49 @@ template <> struct Elt<F16> {
   static __device__ __forceinline__ void store4(F16* p, f32x4 v) { stu(p, u16x4{put(v[0]).u, put(v[1]).u, put(v[2]).u, put(v[3]).u}); }
 };
 
+// 16 bytes of a row at a time: VEC elements, kept packed until they are used
+template <typename T>
+struct Vec16 {
+  static constexpr int N = 16 / sizeof(T);
+  static __device__ __forceinline__ void unpack(u32x4 r, float* x) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(r[i]);
+    } else if constexpr (Elt<T>::id == FRL_ELT_BF16) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(r[i] << 16); x[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u); }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[2 * i] = Elt<T>::get(T{(unsigned short)r[i]});
+        x[2 * i + 1] = Elt<T>::get(T{(unsigned short)(r[i] >> 16)});
+      }
+    }
+  }
+  static __device__ __forceinline__ u32x4 pack(const float* x) {
+    u32x4 r;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[i] = __float_as_uint(x[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (Elt<T>::id == FRL_ELT_BF16) {
+          typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+          r[i] = __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{x[2 * i], x[2 * i + 1]}, bf2));     // v_cvt_pk_bf16_f32
+        } else {
+          r[i] = (unsigned)Elt<T>::put(x[2 * i]).u | (unsigned)Elt<T>::put(x[2 * i + 1]).u << 16;
+        }
+      }
+    }
+    return r;
+  }
+  static __device__ __forceinline__ u32x4 fill_minus_inf() {
+    const unsigned w = sizeof(T) == 4 ? 0xff800000u : Elt<T>::id == FRL_ELT_BF16 ? 0xff80ff80u : 0xfc00fc00u;
+    return u32x4{w, w, w, w};
+  }
+};
+
 __device__ __forceinline__ long long ld_id(const void* p, long long i, int ids64) {
   return ids64 ? ((const long long*)p)[i] : (long long)((const int*)p)[i];
 }
@@ -72,10 +115,12 @@ __device__ __forceinline__ void group_sync() {
   }
 }
 
-__device__ __forceinline__ unsigned long long shfl_xor64(unsigned long long v, int off) {
-  const unsigned lo = __shfl_xor((unsigned)v, off), hi = __shfl_xor((unsigned)(v >> 32), off);
-  return ((unsigned long long)hi << 32) | lo;
+// A grid of any number of workgroups: the second dimension takes over where the first times the workgroup would pass 2^32 threads.
+inline dim3 grid_of(long long blocks) {
+  const long long x = blocks < (1 << 20) ? blocks : (1 << 20);
+  return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
 }
+__device__ __forceinline__ long long block_index() { return (long long)blockIdx.y * gridDim.x + blockIdx.x; }
 
 struct MaxOp {
   static __device__ __forceinline__ float f(float a, float b) { return fmaxf(a, b); }
@@ -85,15 +130,34 @@ struct SumOp {
   template <typename V>
   static __device__ __forceinline__ V f(V a, V b) { return a + b; }
 };
-__device__ __forceinline__ float shfl_x(float v, int off) { return __shfl_xor(v, off); }
-__device__ __forceinline__ double shfl_x(double v, int off) { return __shfl_xor(v, off); }
-__device__ __forceinline__ unsigned long long shfl_x(unsigned long long v, int off) { return shfl_xor64(v, off); }
+// v from another lane of the same row of 16 lanes, by the data-parallel-primitive control CTRL (no LDS traffic)
+template <int CTRL>
+__device__ __forceinline__ unsigned dpp(unsigned v) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true); }
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) { return __uint_as_float(dpp<CTRL>(__float_as_uint(v))); }
+template <int CTRL>
+__device__ __forceinline__ unsigned long long dpp(unsigned long long v) {
+  return ((unsigned long long)dpp<CTRL>((unsigned)(v >> 32)) << 32) | dpp<CTRL>((unsigned)v);
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp(double v) { return __builtin_bit_cast(double, dpp<CTRL>(__builtin_bit_cast(unsigned long long, v))); }
 
+__device__ __forceinline__ unsigned lane_of(unsigned v, int l) { return (unsigned)__builtin_amdgcn_readlane((int)v, l); }
+__device__ __forceinline__ float lane_of(float v, int l) { return __uint_as_float(lane_of(__float_as_uint(v), l)); }
+__device__ __forceinline__ unsigned long long lane_of(unsigned long long v, int l) {
+  return ((unsigned long long)lane_of((unsigned)(v >> 32), l) << 32) | lane_of((unsigned)v, l);
+}
+__device__ __forceinline__ double lane_of(double v, int l) { return __builtin_bit_cast(double, lane_of(__builtin_bit_cast(unsigned long long, v), l)); }
+
+// Over the 64 lanes, all of which have to be active: neighbours, quads and halves of a row of 16 by DPP, then the four rows by lane reads.
+// Every lane gets the result; the order of the operations is fixed.
 template <typename Op, typename V>
 __device__ __forceinline__ V wave_reduce(V v) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) v = Op::f(v, shfl_x(v, off));
-  return v;
+  v = Op::f(v, dpp<0xB1>(v));      // quad_perm 1 0 3 2
+  v = Op::f(v, dpp<0x4E>(v));      // quad_perm 2 3 0 1
+  v = Op::f(v, dpp<0x141>(v));     // row_half_mirror: the other quad of eight
+  v = Op::f(v, dpp<0x140>(v));     // row_mirror: the other eight of the row
+  return Op::f(Op::f(lane_of(v, 0), lane_of(v, 16)), Op::f(lane_of(v, 32), lane_of(v, 48)));
 }
 
 // Every thread of the group gets the result; the order of the operations is fixed.  `red` holds one V per wave of the group

@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 from dataclasses import dataclass
 from typing import Optional, Tuple, Union
 
@@ -63,131 +64,169 @@ class Constraints:
 
 _NO_RULES = Constraints()
 
+# A decoding step's call is as short as its host side.  The C structs are therefore filled with one pack each (their ctypes layout,
+# checked here once) and every operand takes one cheap test on the way to its pointer; only an operand that fails it is looked at closely.
+_DESC, _BUFS = struct.Struct("@4iq4i7q4f"), struct.Struct("@16Q")
+_DDESC, _DBUFS = struct.Struct("@8i5qf4x"), struct.Struct("@8Q")
+for _s, _t in ((_DESC, _lib.FrlLogitsDesc), (_BUFS, _lib.FrlLogitsBufs), (_DDESC, _lib.FrlDistillDesc), (_DBUFS, _lib.FrlDistillBufs)):
+    assert _s.size == C.sizeof(_t), _t
 
-def _check_logits(logits: torch.Tensor, what: str) -> Tuple[torch.Tensor, int, int]:
-    """(rows x vocab view with contiguous rows, rows, vocab)"""
+
+def _check_logits(logits: torch.Tensor, what: str) -> Tuple[torch.Tensor, int, int, int]:
+    """(logits with contiguous rows that do not overlap, rows, vocab, row stride)"""
     if not logits.is_cuda:
         raise RuntimeError("flowrl_hip runs on the GPU only; there is no CPU fallback")
     if logits.dtype not in _ELT:
         raise TypeError(f"{what}: float32, bfloat16 or float16 required (got {logits.dtype})")
-    if logits.dim() < 1 or logits.shape[-1] < 1:
-        raise ValueError(f"{what}: (..., vocab) with at least one entry expected, got {tuple(logits.shape)}")
-    V = logits.shape[-1]
-    z = logits if logits.dim() == 2 else logits.reshape(-1, V) if logits.numel() else logits.reshape(math.prod(logits.shape[:-1]), V)
-    R = z.shape[0]
+    shape = logits.shape
+    if len(shape) < 1 or shape[-1] < 1:
+        raise ValueError(f"{what}: (..., vocab) with at least one entry expected, got {tuple(shape)}")
+    V = shape[-1]
+    R = shape[0] if len(shape) == 2 else math.prod(shape[:-1])
+    if logits.is_contiguous():
+        return logits, R, V, V
+    z = logits if len(shape) == 2 else logits.reshape(R, V)
     if (V > 1 and z.stride(1) != 1) or (R > 1 and z.stride(0) < V):
         z = z.contiguous()
-    return z, R, V
+    return z, R, V, z.stride(0)
 
 
-def _on(t: torch.Tensor, dev: torch.device, what: str) -> torch.Tensor:
-    if t.device != dev:
-        raise ValueError(f"{what}: on {t.device}, expected {dev}")
-    return t
+def _on(t: torch.Tensor, index: int, what: str) -> None:
+    if t.get_device() != index:
+        raise ValueError(f"{what}: on {t.device}, expected device {index}")
 
 
-def _row_values(t: torch.Tensor, R: int, dev: torch.device, dtype: torch.dtype, what: str) -> torch.Tensor:
-    """A tensor of one value per row."""
-    if t.dtype != dtype or t.numel() != R:
+def _row_values(t: torch.Tensor, R: int, index: int, dtype: torch.dtype, what: str) -> torch.Tensor:
+    """A tensor of one value per row, contiguous."""
+    if t.dtype is not dtype or t.numel() != R:
         raise TypeError(f"{what}: {R} values of {dtype} expected (got {tuple(t.shape)} of {t.dtype})")
-    _on(t, dev, what)
-    return t if t.dim() == 1 and (R <= 1 or t.stride(0) == 1) else t.reshape(R).contiguous()
+    if t.get_device() != index:
+        _on(t, index, what)
+    return t if t.is_contiguous() else t.contiguous()
 
 
-def _rows_of(t: torch.Tensor, R: int, n: int, dev: torch.device, what: str, shared: bool) -> Tuple[torch.Tensor, int]:
+def _rows_of(t: torch.Tensor, R: int, n: int, index: int, what: str, shared: bool) -> Tuple[torch.Tensor, int]:
     """(tensor, row stride) of an (n,) or (rows, n) operand; stride 0 where one row serves all."""
-    _on(t, dev, what)
-    if shared and t.dim() == 1 and t.shape[0] == n:
-        return (t if n <= 1 or t.stride(0) == 1 else t.contiguous()), 0
-    if t.dim() < 1 or t.shape[-1] != n or t.numel() != R * n:
-        raise ValueError(f"{what}: ({'' if not shared else f'{n},) or ('}{R}, {n}) expected, got {tuple(t.shape)}")
-    t = t if t.dim() == 2 else t.reshape(R, n)
+    if t.get_device() != index:
+        _on(t, index, what)
+    shape = t.shape
+    if len(shape) == 2 and shape[1] == n and shape[0] == R:
+        if t.is_contiguous():
+            return t, n
+    elif shared and len(shape) == 1 and shape[0] == n:
+        return (t if t.is_contiguous() else t.contiguous()), 0
+    elif len(shape) < 1 or shape[-1] != n or t.numel() != R * n:
+        raise ValueError(f"{what}: ({'' if not shared else f'{n},) or ('}{R}, {n}) expected, got {tuple(shape)}")
+    else:
+        t = t.reshape(R, n)
     if n > 1 and t.stride(1) != 1:
         t = t.contiguous()
     return t, t.stride(0)
 
 
-def _ids(t: torch.Tensor, what: str) -> torch.Tensor:
-    if t.dtype not in (torch.int32, torch.int64):
-        raise TypeError(f"{what}: int32 or int64 tokens required (got {t.dtype})")
-    return t
+def _ids(t: torch.Tensor, what: str) -> int:
+    """1 for int64 tokens, 0 for int32"""
+    if t.dtype is torch.int32:
+        return 0
+    if t.dtype is torch.int64:
+        return 1
+    raise TypeError(f"{what}: int32 or int64 tokens required (got {t.dtype})")
 
 
 def _no_grad(what: str, *ts) -> None:
-    if torch.is_grad_enabled() and any(torch.is_tensor(t) and t.requires_grad for t in ts):
-        raise NotImplementedError(f"flowrl_hip.logits: {what} is not differentiated here; detach it")
+    for t in ts:
+        if t is not None and t.requires_grad:
+            raise NotImplementedError(f"flowrl_hip.logits: {what} is not differentiated here; detach it")
 
 
-def _marshal(z: torch.Tensor, R: int, V: int, c: Constraints):
-    """FrlLogitsDesc / FrlLogitsBufs of one call, and the tensors that they point into."""
-    dev = z.device
-    d, b, keep = _lib.FrlLogitsDesc(), _lib.FrlLogitsBufs(), [z]
-    d.abi_version, d.dtype, d.vocab, d.rows, d.logits_stride = _lib.FRL_ABI_VERSION, _ELT[z.dtype], V, R, z.stride(0)
-    b.logits = z.data_ptr()
-    history, tokens = c.history, c.bias_tokens
-    if history is not None and tokens is not None and history.dtype != tokens.dtype:
-        history, tokens = _ids(history, "history").long(), _ids(tokens, "bias_tokens").long()
+def _marshal(z: torch.Tensor, R: int, V: int, c: Constraints, z_stride: Optional[int] = None, out_elt: int = 0, out_stride: int = 0, out: int = 0,
+             temperature: float = 0.0, temperature_ptr: int = 0, gumbel_stride: int = 0, gumbel: int = 0, token: int = 0, logprob: int = 0):
+    """FrlLogitsDesc / FrlLogitsBufs of one call, and the copies that they point into."""
+    index, keep = z.get_device(), []
+    ids64 = L = K = mask = h_stride = b_stride = s_stride = m_stride = 0
+    h_ptr = b_ptr = t_ptr = v_ptr = a_ptr = 0
+    rows = [0, 0, 0, 0, 0]                  # lengths, prompt_lengths, repetition, frequency, presence
+    rep, freq, pres = 1.0, 0.0, 0.0
+    history, tokens, values = c.history, c.bias_tokens, c.bias_values
+    if history is not None and tokens is not None and history.dtype is not tokens.dtype:
+        _ids(history, "history"), _ids(tokens, "bias_tokens")
+        history, tokens = history.long(), tokens.long()
     if history is not None:
-        L = _ids(history, "history").shape[-1] if history.dim() else 0
-        history, d.history_stride = _rows_of(history, R, L, dev, "history", shared=False)
+        ids64 = _ids(history, "history")
+        L = history.shape[-1] if history.dim() else 0
+        history, h_stride = _rows_of(history, R, L, index, "history", False)
         keep.append(history)
-        d.history_len, d.ids64, b.history = L, int(history.dtype == torch.int64), history.data_ptr()
-        for name in ("lengths", "prompt_lengths"):
-            t = getattr(c, name)
-            if t is not None:
-                t = _row_values(t, R, dev, torch.int32, name)
-                keep.append(t)
-                setattr(b, name, t.data_ptr())
-        for name in ("repetition", "frequency", "presence"):
-            v = getattr(c, name)
-            if torch.is_tensor(v):
-                v = _row_values(v, R, dev, torch.float32, name)
-                keep.append(v)
-                setattr(b, name, v.data_ptr())
-            else:
-                setattr(d, name, float(v))
+        h_ptr = history.data_ptr()
+        if c.lengths is not None:
+            t = _row_values(c.lengths, R, index, torch.int32, "lengths")
+            keep.append(t)
+            rows[0] = t.data_ptr()
+        if c.prompt_lengths is not None:
+            t = _row_values(c.prompt_lengths, R, index, torch.int32, "prompt_lengths")
+            keep.append(t)
+            rows[1] = t.data_ptr()
+        rep, freq, pres = c.repetition, c.frequency, c.presence
+        if isinstance(rep, torch.Tensor):
+            t = _row_values(rep, R, index, torch.float32, "repetition")
+            keep.append(t)
+            rows[2], rep = t.data_ptr(), 1.0
+        if isinstance(freq, torch.Tensor):
+            t = _row_values(freq, R, index, torch.float32, "frequency")
+            keep.append(t)
+            rows[3], freq = t.data_ptr(), 0.0
+        if isinstance(pres, torch.Tensor):
+            t = _row_values(pres, R, index, torch.float32, "presence")
+            keep.append(t)
+            rows[4], pres = t.data_ptr(), 0.0
     elif c.lengths is not None or c.prompt_lengths is not None:
         raise ValueError("lengths / prompt_lengths without a history")
     if c.bias is not None:
-        if c.bias.dtype != torch.float32:
+        if c.bias.dtype is not torch.float32:
             raise TypeError(f"bias: float32 required (got {c.bias.dtype})")
-        t, d.bias_stride = _rows_of(c.bias, R, V, dev, "bias", shared=True)
+        t, b_stride = _rows_of(c.bias, R, V, index, "bias", True)
         keep.append(t)
-        b.bias = t.data_ptr()
-    if (tokens is None) != (c.bias_values is None):
+        b_ptr = t.data_ptr()
+    if (tokens is None) != (values is None):
         raise ValueError("bias_tokens and bias_values come together")
     if tokens is not None:
-        if c.bias_values.dtype != torch.float32 or c.bias_values.shape != tokens.shape:
-            raise TypeError(f"bias_values: float32 of bias_tokens' shape {tuple(tokens.shape)} required (got {tuple(c.bias_values.shape)} of {c.bias_values.dtype})")
-        K = _ids(tokens, "bias_tokens").shape[-1] if tokens.dim() else 0
-        t, d.sparse_stride = _rows_of(tokens, R, K, dev, "bias_tokens", shared=True)
-        u, stride = _rows_of(c.bias_values, R, K, dev, "bias_values", shared=True)
-        if stride != d.sparse_stride:
-            t, u = t.contiguous(), u.contiguous()
-            d.sparse_stride = 0 if t.dim() == 1 else K
-        keep += [t, u]
-        d.n_sparse, d.ids64, b.bias_tokens, b.bias_values = K, int(t.dtype == torch.int64), t.data_ptr(), u.data_ptr()
-    if c.allowed is not None:
-        if c.allowed.dtype == torch.bool:
-            d.mask, n = _lib.FRL_MASK_BYTES, V
-        elif c.allowed.dtype == torch.int32:
-            d.mask, n = _lib.FRL_MASK_WORDS, (V + 31) // 32
+        if values.dtype is not torch.float32 or values.shape != tokens.shape:
+            raise TypeError(f"bias_values: float32 of bias_tokens' shape {tuple(tokens.shape)} required (got {tuple(values.shape)} of {values.dtype})")
+        ids64 = _ids(tokens, "bias_tokens")
+        K = tokens.shape[-1] if tokens.dim() else 0
+        tokens, s_stride = _rows_of(tokens, R, K, index, "bias_tokens", True)
+        values, stride = _rows_of(values, R, K, index, "bias_values", True)
+        if stride != s_stride:
+            tokens, values, s_stride = tokens.contiguous(), values.contiguous(), K
+        keep += (tokens, values)
+        t_ptr, v_ptr = tokens.data_ptr(), values.data_ptr()
+    allowed = c.allowed
+    if allowed is not None:
+        if allowed.dtype is torch.bool:
+            mask, n = _lib.FRL_MASK_BYTES, V
+        elif allowed.dtype is torch.int32:
+            mask, n = _lib.FRL_MASK_WORDS, (V + 31) // 32
         else:
-            raise TypeError(f"allowed: bool entries or int32 words of 32 entries required (got {c.allowed.dtype})")
-        t, d.mask_stride = _rows_of(c.allowed, R, n, dev, "allowed", shared=True)
-        keep.append(t)
-        b.allowed = t.data_ptr()
+            raise TypeError(f"allowed: bool entries or int32 words of 32 entries required (got {allowed.dtype})")
+        allowed, m_stride = _rows_of(allowed, R, n, index, "allowed", True)
+        keep.append(allowed)
+        a_ptr = allowed.data_ptr()
+    d, b = _lib.FrlLogitsDesc(), _lib.FrlLogitsBufs()
+    _DESC.pack_into(d, 0, _lib.FRL_ABI_VERSION, _ELT[z.dtype], out_elt, V, R, ids64, L, K, mask, V if z_stride is None else z_stride, out_stride, gumbel_stride,
+                    h_stride, b_stride, s_stride, m_stride, rep, freq, pres, temperature)
+    _BUFS.pack_into(b, 0, z.data_ptr(), out, h_ptr, *rows, b_ptr, t_ptr, v_ptr, a_ptr, temperature_ptr, gumbel, token, logprob)
     return d, b, keep
 
 
-def _call(fn, dev: torch.device, *args) -> None:
-    """The entry point on dev's current stream, with dev as the current device while it is called."""
-    stream = torch.cuda.current_stream(dev).cuda_stream
-    if torch.cuda.current_device() == dev.index:
-        _lib.check(fn(*args, stream))
+def _call(fn, index: int, *args) -> None:
+    """The entry point on the device's current stream, with the device as the current one while it is called."""
+    stream = torch.cuda.current_stream(index).cuda_stream
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, stream)
     else:
-        with torch.cuda.device(dev):
-            _lib.check(fn(*args, stream))
+        with torch.cuda.device(index):
+            rc = fn(*args, stream)
+    if rc:
+        _lib.check(rc)
 
 
 def constrain(logits: torch.Tensor, rules: Optional[Constraints] = None, *, out: Optional[torch.Tensor] = None,
@@ -195,29 +234,30 @@ def constrain(logits: torch.Tensor, rules: Optional[Constraints] = None, *, out:
     """The logits with ``rules`` applied, in the logits' type or float32 (``out_dtype``), rounded once.  ``out``: where they go, a
     tensor of the logits' shape with contiguous rows; it may be ``logits`` itself."""
     rules = _NO_RULES if rules is None else rules
-    _no_grad("logits / bias", logits, rules.bias, rules.bias_values)
-    z, R, V = _check_logits(logits, "logits")
+    if torch.is_grad_enabled():
+        _no_grad("logits / bias", logits, rules.bias, rules.bias_values)
+    z, R, V, stride = _check_logits(logits, "logits")
+    index = logits.get_device()
     if out is None:
         dtype = logits.dtype if out_dtype is None else out_dtype
         out = torch.empty(logits.shape, dtype=dtype, device=logits.device)
-        o = out.view(R, V)
+        o_stride = V
     else:
-        if out_dtype is not None and out.dtype != out_dtype:
-            raise TypeError(f"out is {out.dtype}, out_dtype {out_dtype}")
+        dtype = out.dtype
+        if out_dtype is not None and dtype != out_dtype:
+            raise TypeError(f"out is {dtype}, out_dtype {out_dtype}")
         if out.shape != logits.shape:
             raise ValueError(f"out: {tuple(logits.shape)} expected, got {tuple(out.shape)}")
-        _on(out, logits.device, "out")
-        if out.dim() > 2 and not out.is_contiguous():
+        _on(out, index, "out")
+        if out.dim() != 2 and not out.is_contiguous():
             raise ValueError("out: contiguous, or two-dimensional with contiguous rows")
-        o = out if out.dim() == 2 else out.view(R, V)
-        if (V > 1 and o.stride(1) != 1) or (R > 1 and o.stride(0) < V):
+        o_stride = V if out.dim() != 2 else out.stride(0)
+        if out.dim() == 2 and ((V > 1 and out.stride(1) != 1) or (R > 1 and o_stride < V)):
             raise ValueError("out: contiguous rows that do not overlap expected")
-    if out.dtype != logits.dtype and out.dtype != torch.float32:
-        raise TypeError(f"constrain: {logits.dtype} logits go to {logits.dtype} or float32, not {out.dtype}")
-    d, b, keep = _marshal(z, R, V, rules)
-    d.out_dtype, d.out_stride, b.out = _ELT[out.dtype], o.stride(0), o.data_ptr()
-    _call(_lib.load().frl_logits_constrain, z.device, C.byref(d), C.byref(b))
-    del keep
+    if dtype != logits.dtype and dtype != torch.float32:
+        raise TypeError(f"constrain: {logits.dtype} logits go to {logits.dtype} or float32, not {dtype}")
+    d, b, keep = _marshal(z, R, V, rules, stride, _ELT[dtype], o_stride, out.data_ptr())
+    _call(_lib.load().frl_logits_constrain, index, C.byref(d), C.byref(b))
     return out
 
 
@@ -230,96 +270,84 @@ def choose(logits: torch.Tensor, rules: Optional[Constraints] = None, *, tempera
     first of equal maxima; NaN counts as the largest.  logprob is log softmax of y (of the constrained logits for a greedy row).  A row
     that the rules leave nothing answers token -1 with logprob -inf."""
     rules = _NO_RULES if rules is None else rules
-    _no_grad("logits / bias", logits, rules.bias, rules.bias_values)
-    z, R, V = _check_logits(logits, "logits")
-    dev = z.device
-    d, b, keep = _marshal(z, R, V, rules)
-    if torch.is_tensor(temperature):
-        t = _row_values(temperature, R, dev, torch.float32, "temperature")
-        keep.append(t)
-        b.temperature = t.data_ptr()
-    else:
-        d.temperature = float(temperature)
+    if torch.is_grad_enabled():
+        _no_grad("logits / bias", logits, rules.bias, rules.bias_values)
+    z, R, V, stride = _check_logits(logits, "logits")
+    index, dev = logits.get_device(), logits.device
+    t = g = None
+    t_ptr = g_ptr = g_stride = 0
+    if isinstance(temperature, torch.Tensor):
+        t = _row_values(temperature, R, index, torch.float32, "temperature")
+        t_ptr, temperature = t.data_ptr(), 0.0
     if gumbel is not None:
-        if gumbel.dtype != torch.float32:
+        if gumbel.dtype is not torch.float32:
             raise TypeError(f"gumbel: float32 required (got {gumbel.dtype})")
-        g, stride = _rows_of(gumbel, R, V, dev, "gumbel", shared=False)
-        if R > 1 and stride < V:
-            g = g.contiguous()
-            stride = V
-        keep.append(g)
-        d.gumbel_stride, b.gumbel = stride, g.data_ptr()
+        g, g_stride = _rows_of(gumbel, R, V, index, "gumbel", False)
+        if R > 1 and g_stride < V:
+            g, g_stride = g.contiguous(), V
+        g_ptr = g.data_ptr()
     lead = logits.shape[:-1]
     token = torch.empty(lead, dtype=torch.int32, device=dev)
     logprob = torch.empty(lead, dtype=torch.float32, device=dev)
-    b.token, b.logprob = token.data_ptr(), logprob.data_ptr()
+    d, b, keep = _marshal(z, R, V, rules, stride, 0, 0, 0, temperature, t_ptr, g_stride, g_ptr, token.data_ptr(), logprob.data_ptr())
     lib = _lib.load()
     # a tensor of this call's own: calls on two streams, and graphs captured from them, share no scratch
     need = lib.frl_logits_workspace_bytes(C.byref(d))
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _call(lib.frl_logits_choose, dev, C.byref(d), C.byref(b), ws.data_ptr() if need else None, need)
-    del keep
+    _call(lib.frl_logits_choose, index, C.byref(d), C.byref(b), ws.data_ptr() if need else None, need)
     return token, logprob
 
 
-def _distill_marshal(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor, kind: str, temperature: float,
-                     weights: Optional[torch.Tensor], reduction: str):
-    if kind not in _KIND:
-        raise ValueError(f"kind {kind!r}: 'logits' or 'logprobs'")
-    if reduction not in _REDUCTION:
-        raise ValueError(f"reduction {reduction!r}: 'mean', 'sum' or 'none'")
-    z, R, V = _check_logits(logits, "logits")
-    dev = z.device
+def _distill_marshal(logits, ids, teacher, kind, temperature, weights, reduction, loss=0, stats=0, g_loss=0, grad=0):
+    """FrlDistillDesc / FrlDistillBufs of one call, its rows, and the copies that they point into."""
+    z, R, V, stride = _check_logits(logits, "logits")
+    index = logits.get_device()
     if teacher.dtype not in _ELT:
         raise TypeError(f"teacher: float32, bfloat16 or float16 required (got {teacher.dtype})")
-    K = _ids(ids, "ids").shape[-1] if ids.dim() else 0
+    ids64 = _ids(ids, "ids")
+    K = ids.shape[-1] if ids.dim() else 0
     if K < 1:
         raise ValueError(f"ids: (rows, top) with at least one entry expected, got {tuple(ids.shape)}")
+    i, i_stride = _rows_of(ids, R, K, index, "ids", False)
+    t, t_stride = _rows_of(teacher, R, K, index, "teacher", False)
+    w = None if weights is None else _row_values(weights, R, index, torch.float32, "weights")
     d, b = _lib.FrlDistillDesc(), _lib.FrlDistillBufs()
-    i, d.ids_stride = _rows_of(ids, R, K, dev, "ids", shared=False)
-    t, d.teacher_stride = _rows_of(teacher, R, K, dev, "teacher", shared=False)
-    d.abi_version, d.dtype, d.teacher_dtype, d.ids64 = _lib.FRL_ABI_VERSION, _ELT[z.dtype], _ELT[t.dtype], int(i.dtype == torch.int64)
-    d.kind, d.reduction, d.vocab, d.top, d.rows = _KIND[kind], _REDUCTION[reduction], V, K, R
-    d.logits_stride, d.temperature = z.stride(0), float(temperature)
-    b.logits, b.ids, b.teacher = z.data_ptr(), i.data_ptr(), t.data_ptr()
-    keep = [z, i, t]
-    if weights is not None:
-        w = _row_values(weights, R, dev, torch.float32, "weights")
-        keep.append(w)
-        b.weights = w.data_ptr()
-    return d, b, keep
+    _DDESC.pack_into(d, 0, _lib.FRL_ABI_VERSION, _ELT[z.dtype], _ELT[t.dtype], ids64, _KIND[kind], _REDUCTION[reduction], V, K, R, stride, V, i_stride, t_stride, temperature)
+    _DBUFS.pack_into(b, 0, z.data_ptr(), i.data_ptr(), t.data_ptr(), 0 if w is None else w.data_ptr(), loss, stats, g_loss, grad)
+    return d, b, (z, i, t, w)
 
 
 def distill_forward(logits, ids, teacher, kind, temperature, weights, reduction, want_grad=False, want_stats=False):
     """(loss, grad or None, row statistics or None): frl_distill_fwd."""
-    d, b, keep = _distill_marshal(logits, ids, teacher, kind, temperature, weights, reduction)
-    dev, R, V = logits.device, d.rows, d.vocab
-    loss = torch.empty(logits.shape[:-1] if reduction == "none" else (), dtype=torch.float32, device=dev)
+    if kind not in _KIND:
+        raise ValueError(f"kind {kind!r}: 'logits' or 'logprobs'")
+    if reduction not in _REDUCTION:
+        raise ValueError(f"reduction {reduction!r}: 'mean', 'sum' or 'none'")
+    if not logits.is_cuda:
+        raise RuntimeError("flowrl_hip runs on the GPU only; there is no CPU fallback")
+    dev, lead = logits.device, logits.shape[:-1]
+    loss = torch.empty(lead if reduction == "none" else (), dtype=torch.float32, device=dev)
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if want_grad else None
-    stats = torch.empty((R + 1, _lib.FRL_DISTILL_STATS), dtype=torch.float32, device=dev) if want_stats else None
-    b.loss = loss.data_ptr()
-    if R == 0 and reduction == "none":
+    stats = torch.empty((math.prod(lead) + 1, _lib.FRL_DISTILL_STATS), dtype=torch.float32, device=dev) if want_stats else None
+    d, b, keep = _distill_marshal(logits, ids, teacher, kind, temperature, weights, reduction, loss.data_ptr(), stats.data_ptr() if want_stats else 0, 0,
+                                  grad.data_ptr() if want_grad else 0)
+    if reduction == "none" and loss.numel() == 0:
         return loss, grad, stats
-    if want_grad:
-        b.grad, d.grad_stride = grad.data_ptr() or None, V
-    if want_stats:
-        b.row_stats = stats.data_ptr()
     lib = _lib.load()
     need = lib.frl_distill_workspace_bytes(C.byref(d))
-    ws = torch.empty(max(need, 256), dtype=torch.uint8, device=dev)
-    _call(lib.frl_distill_fwd, dev, C.byref(d), C.byref(b), ws.data_ptr(), ws.numel())
-    del keep
+    ws = torch.empty(need or 256, dtype=torch.uint8, device=dev)       # need == 0: the entry point says why
+    _call(lib.frl_distill_fwd, logits.get_device(), C.byref(d), C.byref(b), ws.data_ptr(), need)
     return loss, grad, stats
 
 
 def distill_backward(logits, ids, teacher, kind, temperature, weights, reduction, stats, g_loss):
     """d loss / d logits times ``g_loss`` from the forward's row statistics: frl_distill_bwd."""
-    d, b, keep = _distill_marshal(logits, ids, teacher, kind, temperature, weights, reduction)
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    g = _row_values(g_loss, d.rows if reduction == "none" else 1, logits.device, torch.float32, "g_loss")
-    b.row_stats, b.g_loss, b.grad, d.grad_stride = stats.data_ptr(), g.data_ptr(), grad.data_ptr(), d.vocab
-    _call(_lib.load().frl_distill_bwd, logits.device, C.byref(d), C.byref(b))
-    del keep
+    index = logits.get_device()
+    g = _row_values(g_loss, math.prod(logits.shape[:-1]) if reduction == "none" else 1, index, torch.float32, "g_loss")
+    d, b, keep = _distill_marshal(logits, ids, teacher, kind, temperature, weights, reduction, 0, stats.data_ptr(), g.data_ptr(), grad.data_ptr())
+    if grad.numel():
+        _call(_lib.load().frl_distill_bwd, index, C.byref(d), C.byref(b))
     return grad
 
 
@@ -334,6 +362,7 @@ def distill_loss(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor,
     ``weights`` (rows,) float32: a row of weight 0 is not read.  ``reduction`` "mean" divides by the sum of the weights; "none" returns
     the rows' weighted divergences.  With ``want_grad`` also d loss / d logits in the logits' type, in the same pass ("none": of
     the rows' sum).  Like ``mse_loss`` a value without a graph; :func:`flowrl_hip.autograd.distill_loss` differentiates."""
-    _no_grad("logits (use flowrl_hip.autograd.distill_loss) / teacher / weights", logits, teacher, weights)
+    if torch.is_grad_enabled():
+        _no_grad("logits (use flowrl_hip.autograd.distill_loss) / teacher / weights", logits, teacher, weights)
     loss, grad, _ = distill_forward(logits, ids, teacher, kind, temperature, weights, reduction, want_grad)
     return (loss, grad) if want_grad else loss
