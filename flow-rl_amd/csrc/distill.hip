@@ -14,9 +14,6 @@
 // Rows beyond that, or too few to fill the chip, are split over their length, joined by a second kernel, and differentiated by a third.
 #include "frl_rows.h"
 
-// No product is fused into a sum but where the code says so: the kernels that share the code below then round alike.
-#pragma clang fp contract(off)
-
 namespace frl {
 
 struct DistillArgs {
@@ -32,6 +29,7 @@ struct DistillArgs {
   int vocab, top, ids64, teacher_dtype, segs, seg_len, g_stride;
 };
 
+constexpr double LN2 = 0.6931471805599453;
 constexpr int DSEG_MAX = 1 << 16;      // entries of a segment
 constexpr int DROW_MAX = 1 << 18;      // entries of a row that is not split
 
@@ -52,24 +50,6 @@ __device__ __forceinline__ void mark_named(const DistillArgs& a, long long row, 
   }
   group_sync<G>();
 }
-
-// 2^((x - m) c).  With a finite product M = m c this is one fma, whose rounding of M shifts every exponent of the row alike; a maximum near
-// the type's lowest value (a row masked throughout) takes the difference first.
-struct Shift {
-  float m, M, c;
-  bool fast;
-  __device__ __forceinline__ Shift(float m_, float c_) : m(m_), M(m_ * c_), c(c_) { fast = fabsf(M) < INFINITY; }
-  template <int N>
-  __device__ __forceinline__ void exps(float* x) const {
-    if (fast) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], c, -M));
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) x[i] = __builtin_amdgcn_exp2f((x[i] - m) * c);
-    }
-  }
-};
 
 template <int N>
 __device__ __forceinline__ float max_of(const float* x, float m) {
@@ -102,9 +82,7 @@ struct Running {
   float m = -INFINITY, s = 0.0f, r = 0.0f;
   __device__ __forceinline__ void raise(float to, float c) {
     if (to > m) {
-      const float f = __builtin_amdgcn_exp2f((m - to) * c);
-      s *= f;
-      r *= f;
+      about(to, c);
       m = to;
     }
   }
@@ -148,7 +126,7 @@ struct Running {
   // the sums with respect to a maximum over more threads; a thread that saw only -inf has sums of 0 (or NaN) and keeps them
   __device__ __forceinline__ void about(float all, float c) {
     if (m != -INFINITY) {
-      const float f = __builtin_amdgcn_exp2f((m - all) * c);
+      const float f = Shift(all, c).from(Shift(m, c));
       s *= f;
       r *= f;
     }
@@ -182,7 +160,7 @@ __device__ __forceinline__ void teacher_part(const DistillArgs& a, long long row
     if (valid) {
       const float t = teacher_at(a.teacher, row * a.teacher_stride + k, a.teacher_dtype);
       zk = Elt<T>::get(z[id]);
-      const float y = zk * a.inv_temp;
+      const double y = (double)zk * (double)a.scale2 * LN2;      // with the rounded log2(e) / T of the exponentials: one temperature throughout
       float lp;
       if constexpr (REST) {
         const double pd = exp((double)t);
@@ -195,7 +173,7 @@ __device__ __forceinline__ void teacher_part(const DistillArgs& a, long long row
         lp = d - log_tot;
         sum_p += (double)p;
       }
-      if (p != 0.0f) cross += (double)p * ((double)lp - (double)y);
+      if (p != 0.0f) cross += (double)p * ((double)lp - y);
     }
     sid[k] = valid ? (int)id : -1;
     sp[k] = p;
@@ -227,7 +205,8 @@ __device__ __forceinline__ Factors row_factors(float s, float r, double sum_p) {
 template <bool REST>
 __device__ __forceinline__ float row_loss(const DistillArgs& a, float m, float s, float r, double sum_p, double cross) {
   if (!REST && sum_p == 0.0) return 0.0f;
-  double loss = cross + sum_p * ((double)m * (double)a.inv_temp + log((double)s));
+  const Shift sh(m, a.scale2);
+  double loss = cross + sum_p * ((sh.fast ? (double)sh.M : (double)m * (double)a.scale2) * LN2 + log((double)s));
   if constexpr (REST) {
     const double P = 1.0 - sum_p;
     if (P > 0.0) loss += P * log(P * (double)s / (double)r);
@@ -311,13 +290,6 @@ template <int NV>
 __device__ __forceinline__ void keep_packed(u32x4* raw) {
 #pragma unroll
   for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(raw[i]));
-}
-
-// The thread's number as a value of its own: what is derived from it, an index and an address per vector, is then computed where it is used and not
-// kept in registers across the passes and rows.
-__device__ __forceinline__ int fresh(int tid) {
-  asm volatile("" : "+v"(tid));
-  return tid;
 }
 
 // A row to a group, its first NV vectors per thread held in registers: value, what the backward needs, and (GRAD) the gradient.

@@ -4,6 +4,10 @@
 
 #include "frl_device.h"
 
+// No product is fused into a sum but where the code says so (also for what follows in the including file): results do not depend on
+// which products the compiler fuses in which kernel.
+#pragma clang fp contract(off)
+
 namespace frl {
 
 void clear_kernels();      // capi.hip: frl_last_kernels starts anew
@@ -114,6 +118,35 @@ __device__ __forceinline__ void group_sync() {
     __syncthreads();
   }
 }
+
+// The thread's number as a value of its own: what is derived from it, an index and an address per vector, is then computed where it is used and not
+// kept in registers across the passes and rows.
+__device__ __forceinline__ int fresh(int tid) {
+  asm volatile("" : "+v"(tid));
+  return tid;
+}
+
+// 2^((x - m) c).  With a finite product M = m c this is one fma, whose rounding of M shifts every exponent of the row alike; a maximum near
+// the type's lowest value (a row masked throughout) takes the difference first.
+struct Shift {
+  float m, M, c;
+  bool fast;
+  __device__ __forceinline__ Shift(float m_, float c_) : m(m_), M(m_ * c_), c(c_) { fast = fabsf(M) < INFINITY; }
+  template <int N>
+  __device__ __forceinline__ void exps(float* x) const {
+    if (fast) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], c, -M));
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = __builtin_amdgcn_exp2f((x[i] - m) * c);
+    }
+  }
+  // the factor that turns a sum with another, lower shift into one with this: the same rounded products as the exponentials', so they cancel
+  __device__ __forceinline__ float from(const Shift& o) const {
+    return __builtin_amdgcn_exp2f(fast && o.fast ? o.M - M : (o.m - m) * c);
+  }
+};
 
 // A grid of any number of workgroups: the second dimension takes over where the first times the workgroup would pass 2^32 threads.
 inline dim3 grid_of(long long blocks) {

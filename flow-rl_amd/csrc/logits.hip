@@ -5,9 +5,11 @@
 // argmax of key and y[token] - log sum exp y from a maximum and a sum.
 //
 // HBM-bound: an element is read once (and, choose, its noise), a result written once.  What must not cost a pass over the
-// vocabulary of its own is the history, a list of tokens.  A group of G threads therefore owns a chunk of 8 G entries
-// of one row: it counts the tokens of the history that fall into its chunk in LDS (integer adds: any order gives the same counts),
-// sums the listed biases there, and applies both to the logits that it loaded into registers before it began.
+// vocabulary of its own is the lists, a history of tokens and biases by token.  A group of G threads (a wave up to a workgroup of 1024) takes
+// consecutive chunks of 8 G entries of one row.  For each it counts the history's tokens that fall into the chunk in one LDS word per entry
+// (integer adds: any order gives the same counts), puts the number of a listed bias beside the count, and applies both to the
+// logits, which are on their way meanwhile.  Two sets of words take turns, so a chunk costs one barrier; a choice keeps its maximum and sum in
+// registers from chunk to chunk and reduces them once.
 #include "frl_rows.h"
 
 namespace frl {
@@ -20,11 +22,19 @@ struct LogitsArgs {
   unsigned long long* part_key; float* part_m; float* part_s; float* part_y;   // choose over several chunks: one entry per (row, chunk)
   long long logits_stride, out_stride, gumbel_stride, history_stride, bias_stride, sparse_stride, mask_stride;
   float rep, freq, pres, temp;
-  unsigned items, chunks;
   int vocab, ids64, L, K, mask;
+  long long items;          // rows x parts
+  int chunks, per, parts;   // of a row: chunks of 8 G entries, `per` of them to a part (one group's work)
 };
 
+// One LDS word per entry of a chunk: bit 31 the token stands in the prompt; bits 19..30 one more than the slot of its listed bias, 0 for none;
+// bits 0..18 how often it was generated.  Without listed biases the count has all 31 bits.
 constexpr unsigned SEEN_IN_PROMPT = 0x80000000u;
+constexpr int SLOT_SHIFT = 19;
+constexpr unsigned COUNT_MASK = (1u << SLOT_SHIFT) - 1u, SLOT_MASK = 0xfffu;
+constexpr int MAX_HISTORY_WITH_SLOTS = (1 << SLOT_SHIFT) - 1;
+constexpr int HIST_REGS = 4;                               // history entries a thread keeps; longer histories are read again for every chunk
+constexpr unsigned NO_TOKEN = 0x7fffffffu;                 // beyond every vocabulary (at most 2^30) from any chunk's first entry
 
 // key as an unsigned number in argmax's order (a NaN above everything, -0 equal to +0), then the index so that the lower wins
 __device__ __forceinline__ unsigned long long key_of(float key, unsigned v) {
@@ -33,61 +43,73 @@ __device__ __forceinline__ unsigned long long key_of(float key, unsigned v) {
   return ((unsigned long long)o << 32) | (unsigned)~v;
 }
 
-// the chunk's counts: history entries t of [0, len), the first `plen` of them prompt
-template <int G>
-__device__ __forceinline__ void count_history(const LogitsArgs& a, long long row, int tid, unsigned v0, unsigned n, unsigned* cnt) {
-  int len = a.L, plen = 0;
-  if (a.lengths != nullptr) len = min(max(a.lengths[row], 0), a.L);
-  if (a.prompt_lengths != nullptr) plen = min(max(a.prompt_lengths[row], 0), len);
-  auto count = [&](unsigned long long id, int t) {
-    const unsigned long long loc = id - v0;                 // a token below the chunk wraps round and is out of range too
-    if (loc < n) {
-      if (t < plen) atomicOr(&cnt[loc], SEEN_IN_PROMPT);
-      else atomicAdd(&cnt[loc], 1u);
-    }
-  };
-  if (a.ids64) {
-    const long long* h = (const long long*)a.history + row * a.history_stride;
-#pragma unroll 4
-    for (int t = tid; t < len; t += G) count((unsigned long long)h[t], t);
-  } else {
-    const int* h = (const int*)a.history + row * a.history_stride;
-#pragma unroll 4
-    for (int t = tid; t < len; t += G) count((unsigned long long)(long long)h[t], t);
+// x / d with r = 1 / d: the quotient's error is brought back in by one fma (Markstein), which leaves the correctly rounded quotient but
+// where it is subnormal; an infinite quotient stays
+__device__ __forceinline__ float divide(float x, float d, float r) {
+  const float q = x * r;
+  const float q2 = __builtin_fmaf(__builtin_fmaf(-q, d, x), r, q);
+  return q2 == q2 ? q2 : q;
+}
+
+// Entry t of the history: its token (NO_TOKEN for padding), bit 31 set in the prompt
+__device__ __forceinline__ unsigned history_entry(const LogitsArgs& a, const void* h, int t, int plen) {
+  const long long id = ld_id(h, t, a.ids64);
+  return id >= 0 && id < a.vocab ? (unsigned)id | (t < plen ? SEEN_IN_PROMPT : 0u) : NO_TOKEN;
+}
+
+__device__ __forceinline__ void count_entry(unsigned e, unsigned v0, unsigned n, unsigned* cnt) {
+  const unsigned loc = (e & ~SEEN_IN_PROMPT) - v0;          // tokens below the chunk wrap round and are out of range too
+  if (loc < n) {
+    if (e & SEEN_IN_PROMPT) atomicOr(&cnt[loc], SEEN_IN_PROMPT);
+    else atomicAdd(&cnt[loc], 1u);
   }
 }
 
-// Listed biases, summed per token in the order of the list whatever threads hold them: a first pass counts how many entries
-// name a token, a lone entry then stores its value, and of several the first one sums them all.
+// The row's listed biases, once: tokens and values into LDS, a token named several times summed in the order of the list into its first
+// entry (the others become NO_TOKEN).  Whether any is, a table of the tokens finds out; `table` is the chunks' words, free and zero before and after.
 template <int G>
-__device__ __forceinline__ void mark_listed(const LogitsArgs& a, long long row, int tid, unsigned v0, unsigned n, int* add) {
-  for (int k = tid; k < a.K; k += G) {
-    const unsigned long long loc = (unsigned long long)ld_id(a.bias_tokens, row * a.sparse_stride + k, a.ids64) - v0;
-    if (loc < n) atomicAdd(&add[loc], 1);
-  }
-}
-template <int G>
-__device__ __forceinline__ void sum_listed(const LogitsArgs& a, long long row, int tid, unsigned v0, unsigned n, float* add) {
+__device__ __forceinline__ void stage_listed(const LogitsArgs& a, long long row, int tid, unsigned* table, unsigned* tok, float* val, int* several) {
+  constexpr unsigned SLOTS = 8 * G;                        // a power of two
   const long long at = row * a.sparse_stride;
-  unsigned several = 0;                                      // bit i: this thread's entry i shares its token (K <= 2048: at most 32 entries)
-  for (int k = tid, i = 0; k < a.K; k += G, ++i) {
-    const unsigned long long loc = (unsigned long long)ld_id(a.bias_tokens, at + k, a.ids64) - v0;
-    if (loc < n && ((const int*)add)[loc] > 1) several |= 1u << i;
-  }
-  group_sync<G>();                                           // every count is read before a value takes its place
-  for (int k = tid, i = 0; k < a.K; k += G, ++i) {
+  if (tid == 0) *several = a.K > (int)SLOTS / 2;
+  for (int k = tid; k < a.K; k += G) {
     const long long id = ld_id(a.bias_tokens, at + k, a.ids64);
-    const unsigned long long loc = (unsigned long long)id - v0;
-    if (loc >= n) continue;
-    float s = a.bias_values[at + k];
-    if (several >> i & 1u) {
-      bool first = true;
-      for (int j = 0; j < k && first; ++j) first = ld_id(a.bias_tokens, at + j, a.ids64) != id;
-      if (!first) continue;
-      for (int j = k + 1; j < a.K; ++j)
-        if (ld_id(a.bias_tokens, at + j, a.ids64) == id) s += a.bias_values[at + j];
+    tok[k] = id >= 0 && id < a.vocab ? (unsigned)id : NO_TOKEN;
+    val[k] = a.bias_values[at + k];
+  }
+  group_sync<G>();
+  if (a.K <= (int)SLOTS / 2) {                             // at most half full: a free slot is always found
+    for (int k = tid; k < a.K; k += G) {
+      if (tok[k] == NO_TOKEN) continue;
+      const unsigned mine = tok[k] + 1u;
+      for (unsigned i = mine * 2654435761u, probe = 0; probe < SLOTS; ++probe, ++i) {
+        const unsigned was = atomicCAS(&table[i % SLOTS], 0u, mine);
+        if (was == mine) *several = 1;
+        if (was == 0u || was == mine) break;
+      }
     }
-    add[loc] = s;
+    group_sync<G>();
+#pragma unroll
+    for (int q = 0; q < 2; ++q) *(i32x4*)(table + q * 4 * G + 4 * tid) = i32x4{0, 0, 0, 0};
+  }
+  group_sync<G>();
+  if (*several != 0) {
+    unsigned drop = 0;                                     // bit i: this thread's entry i is not its token's first (K <= 2048: at most 32 entries)
+    for (int k = tid, i = 0; k < a.K; k += G, ++i) {
+      const unsigned t = tok[k];
+      if (t == NO_TOKEN) continue;
+      bool first = true;
+      for (int j = 0; j < k && first; ++j) first = tok[j] != t;
+      if (!first) { drop |= 1u << i; continue; }
+      float s = a.bias_values[at + k];
+      for (int j = k + 1; j < a.K; ++j)
+        if (tok[j] == t) s += a.bias_values[at + j];
+      val[k] = s;
+    }
+    group_sync<G>();
+    for (int k = tid, i = 0; k < a.K; k += G, ++i)
+      if (drop >> i & 1u) tok[k] = NO_TOKEN;
+    group_sync<G>();
   }
 }
 
@@ -119,103 +141,172 @@ __device__ __forceinline__ f32x4 load_quad(const T* p, int left, float fill) {
   return v;
 }
 
+// The running answer of a thread over its entries, in index order: the best key and where, its y, and the sum of exponentials
+struct Choice {
+  float key = -INFINITY, y = -INFINITY, m = -INFINITY, s = 0.0f;
+  unsigned v = 0xffffffffu;
+  bool nan = false;         // v is its first NaN
+};
+constexpr float LOG2E = 1.4426950408889634f;
+
+// what the chunks of a row that one group took come to, in the join's terms
+__device__ __forceinline__ void answer(const LogitsArgs& a, long long row, unsigned long long best, float m, float s, float y) {
+  a.token[row] = best != 0 ? (int32_t) ~(unsigned)best : -1;
+  if (a.logprob == nullptr) return;
+  const Shift sh(m, LOG2E);
+  const float d = sh.fast ? __builtin_fmaf(y, LOG2E, -sh.M) : (y - m) * LOG2E;
+  a.logprob[row] = best != 0 ? (d - __builtin_amdgcn_logf(s)) * 0.69314718f : -INFINITY;
+}
+
+// Four elements as they lie in memory: a two-byte type keeps them in two registers until they are used.
+template <typename T>
+struct Packed4 {
+  u32x2 r;
+  __device__ __forceinline__ void load(const T* p, int left) {
+    if (left >= 4) { r = ldu<u32x2>(p); return; }
+    const unsigned ninf = Elt<T>::put(-INFINITY).u;
+    const unsigned e0 = left > 0 ? p[0].u : ninf, e1 = left > 1 ? p[1].u : ninf, e2 = left > 2 ? p[2].u : ninf;
+    r = u32x2{e0 | e1 << 16, e2 | ninf << 16};
+  }
+  __device__ __forceinline__ void none() { const unsigned ninf = Elt<T>::put(-INFINITY).u; r = u32x2{ninf | ninf << 16, ninf | ninf << 16}; }
+  __device__ __forceinline__ f32x4 get() const {
+    return f32x4{Elt<T>::get(T{(unsigned short)r[0]}), Elt<T>::get(T{(unsigned short)(r[0] >> 16)}),
+                 Elt<T>::get(T{(unsigned short)r[1]}), Elt<T>::get(T{(unsigned short)(r[1] >> 16)})};
+  }
+};
+template <>
+struct Packed4<float> {
+  f32x4 r;
+  __device__ __forceinline__ void load(const float* p, int left) { r = load_quad(p, left, -INFINITY); }
+  __device__ __forceinline__ void none() { r = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY}; }
+  __device__ __forceinline__ f32x4 get() const { return r; }
+};
+
 template <typename T, typename O, int G, bool HIST, bool SPARSE, bool CHOOSE>
-__global__ void __launch_bounds__(G == 64 ? 256 : G) frl_logits_kernel(const LogitsArgs a) {
-#pragma clang fp contract(off)      // each operation rounded on its own: results do not depend on which products the compiler fuses
+__global__ void __launch_bounds__(G == 64 ? 256 : G, 8) frl_logits_kernel(const LogitsArgs a) {
   constexpr int CH = 8 * G, GPB = G == 64 ? 4 : 1;
-  __shared__ __align__(16) unsigned cnt_all[HIST ? GPB * CH : 4];
-  __shared__ __align__(16) float add_all[SPARSE ? GPB * CH : 4];
+  constexpr bool WORDS = HIST || SPARSE;
+  __shared__ __align__(16) unsigned cnt_all[WORDS ? GPB * 2 * CH : 4];
+  extern __shared__ __align__(16) unsigned lists[];         // tokens, then values, of the listed biases
+  __shared__ int several_all[GPB];
   __shared__ unsigned long long red_k[G / 64];
   __shared__ float red_m[G / 64], red_s[G / 64];
-  const int tid = threadIdx.x % G, grp = threadIdx.x / G;
-  unsigned* cnt = cnt_all + (HIST ? grp * CH : 0);
-  float* add = add_all + (SPARSE ? grp * CH : 0);
+  const int tid = threadIdx.x % G, grp = G == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+  unsigned* cnt = cnt_all + (WORDS ? grp * 2 * CH : 0);
+  unsigned* tok = lists + (SPARSE ? grp * 2 * a.K : 0);
+  float* val = (float*)(tok + (SPARSE ? a.K : 0));
   const float NINF = -INFINITY;
 
-  for (unsigned item = blockIdx.x * GPB + grp; item < a.items; item += gridDim.x * GPB) {
-    const long long row = item / a.chunks;
-    const unsigned v0 = (item - (unsigned)row * a.chunks) * CH;
-    const unsigned n = min((unsigned)a.vocab - v0, (unsigned)CH);
-    const float temp = !CHOOSE ? 0.0f : a.temperature != nullptr ? a.temperature[row] : a.temp;
-    const bool sampled = CHOOSE && a.gumbel != nullptr && temp > 0.0f;
-    unsigned bits[2];
-    f32x4 x[2], g[2], b[2];
+  const long long item = block_index() * GPB + grp;
+  if (item >= a.items) return;
+  const long long row = item / a.parts;
+  const int part = (int)(item - row * a.parts);
+  const int c0 = part * a.per, c1 = min(c0 + a.per, a.chunks);
+  const T* z = (const T*)a.logits + row * a.logits_stride;
+  const float temp = !CHOOSE ? 0.0f : a.temperature != nullptr ? a.temperature[row] : a.temp;
+  const bool sampled = CHOOSE && a.gumbel != nullptr && temp > 0.0f;
+  const float inv = sampled ? 1.0f / (1e-6f + temp) : 1.0f;
+  const float* noise = sampled ? a.gumbel + row * a.gumbel_stride : nullptr;
+
+  auto bits_of = [&](int c, int q, int t) -> unsigned {
+    const int v = c * CH + q * 4 * G + 4 * t, left = a.vocab - v;
+    if (left <= 0 || c >= c1) return 0u;
+    unsigned b = a.mask != FRL_MASK_NONE ? allowed4(a, row, v) : 15u;
+    return left < 4 ? b & ((1u << left) - 1u) : b;
+  };
+  unsigned bits[2] = {bits_of(c0, 0, tid), bits_of(c0, 1, tid)};
+
+  int len = 0, plen = 0;
+  unsigned mine[HIST ? HIST_REGS : 1];
+  float rep = 1.0f, rrep = 1.0f, freq = 0.0f, pres = 0.0f;
+  const void* h = nullptr;
+  if constexpr (HIST) {
+    h = (const char*)a.history + row * a.history_stride * (a.ids64 ? 8 : 4);
+    len = a.lengths != nullptr ? min(max(a.lengths[row], 0), a.L) : a.L;
+    plen = a.prompt_lengths != nullptr ? min(max(a.prompt_lengths[row], 0), len) : 0;
+#pragma unroll
+    for (int i = 0; i < HIST_REGS; ++i) mine[i] = tid + i * G < len ? history_entry(a, h, tid + i * G, plen) : NO_TOKEN;
+    rep = a.repetition != nullptr ? a.repetition[row] : a.rep;
+    freq = a.frequency != nullptr ? a.frequency[row] : a.freq;
+    pres = a.presence != nullptr ? a.presence[row] : a.pres;
+    rrep = 1.0f / rep;
+  }
+  if constexpr (WORDS) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) *(i32x4*)(cnt + q * 4 * G + 4 * tid) = i32x4{0, 0, 0, 0};
+    if constexpr (SPARSE) stage_listed<G>(a, row, tid, cnt, tok, val, several_all + grp);
+    group_sync<G>();
+  }
+
+  Choice ch;
+  for (int c = c0; c < c1; ++c) {
+    const int t0 = fresh(tid);
+    const unsigned v0 = (unsigned)c * CH, n = min((unsigned)a.vocab - v0, (unsigned)CH);
+    Packed4<T> raw[2];
+    f32x4 g[2];
     // everything that streams is asked for first; a quad of which nothing is allowed is not read at all
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      const unsigned v = v0 + q * 4 * G + 4 * tid;
+      const unsigned v = v0 + q * 4 * G + 4 * t0;
       const int left = a.vocab - (int)v;
-      bits[q] = left <= 0 ? 0u : a.mask != FRL_MASK_NONE ? allowed4(a, row, v) : 15u;
-      if (left < 4 && left > 0) bits[q] &= (1u << left) - 1u;
-    }
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const unsigned v = v0 + q * 4 * G + 4 * tid;
-      const int left = a.vocab - (int)v;
-      x[q] = f32x4{NINF, NINF, NINF, NINF};
-      g[q] = b[q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      raw[q].none();
+      g[q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       if (bits[q] != 0u) {
-        x[q] = load_quad((const T*)a.logits + row * a.logits_stride + v, left, NINF);
-        if (sampled) g[q] = load_quad(a.gumbel + row * a.gumbel_stride + v, left, 0.0f);
-        if (a.bias != nullptr) b[q] = load_quad(a.bias + row * a.bias_stride + v, left, 0.0f);
+        raw[q].load(z + v, left);
+        if (sampled) g[q] = load_quad(noise + v, left, 0.0f);
       }
     }
-    if constexpr (HIST || SPARSE) {
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        if constexpr (HIST) *(i32x4*)(cnt + q * 4 * G + 4 * tid) = i32x4{0, 0, 0, 0};
-        if constexpr (SPARSE) *(f32x4*)(add + q * 4 * G + 4 * tid) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      }
-      group_sync<G>();
-      if constexpr (SPARSE) mark_listed<G>(a, row, tid, v0, n, (int*)add);
-      if constexpr (HIST) count_history<G>(a, row, tid, v0, n, cnt);
-      group_sync<G>();
-      if constexpr (SPARSE) {
-        sum_listed<G>(a, row, tid, v0, n, add);
-        group_sync<G>();
-      }
+    const unsigned now[2] = {bits[0], bits[1]};
+    if (a.mask != FRL_MASK_NONE || c + 2 >= c1) {
+      bits[0] = bits_of(c + 1, 0, t0);
+      bits[1] = bits_of(c + 1, 1, t0);
     }
-    float rep = 1.0f, freq = 0.0f, pres = 0.0f;
+    unsigned* w = cnt + (WORDS ? ((c - c0) & 1) * CH : 0);
     if constexpr (HIST) {
-      rep = a.repetition != nullptr ? a.repetition[row] : a.rep;
-      freq = a.frequency != nullptr ? a.frequency[row] : a.freq;
-      pres = a.presence != nullptr ? a.presence[row] : a.pres;
+#pragma unroll
+      for (int i = 0; i < HIST_REGS; ++i) count_entry(mine[i], v0, n, w);
+      for (int t = t0 + HIST_REGS * G; t < len; t += G) count_entry(history_entry(a, h, t, plen), v0, n, w);
     }
-    const float inv = sampled ? 1.0f / (1e-6f + temp) : 1.0f;
-    unsigned long long best = 0;
-    float m = NINF;
+    if constexpr (SPARSE) {
+      for (int k = t0; k < a.K; k += G) {
+        const unsigned loc = tok[k] - v0;
+        if (loc < n) atomicAdd(&w[loc], (unsigned)(k + 1) << SLOT_SHIFT);
+      }
+    }
+    f32x4 x[2];
+    float bm = ch.m;
+    if constexpr (WORDS) group_sync<G>();                   // the words are complete; the other set was cleared by the threads that read it
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      const unsigned v = v0 + q * 4 * G + 4 * tid;
-      i32x4 c4 = {0, 0, 0, 0};
-      f32x4 a4 = {0.0f, 0.0f, 0.0f, 0.0f};
-      if constexpr (HIST) c4 = *(const i32x4*)(cnt + q * 4 * G + 4 * tid);
-      if constexpr (SPARSE) a4 = *(const f32x4*)(add + q * 4 * G + 4 * tid);
+      const unsigned v = v0 + q * 4 * G + 4 * t0;
+      const int left = a.vocab - (int)v;
+      x[q] = raw[q].get();
+      i32x4 w4 = {0, 0, 0, 0};
+      if constexpr (WORDS) {
+        w4 = *(const i32x4*)(w + q * 4 * G + 4 * t0);
+        *(i32x4*)(w + q * 4 * G + 4 * t0) = i32x4{0, 0, 0, 0};
+      }
+      f32x4 b = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (a.bias != nullptr && now[q] != 0u) b = load_quad(a.bias + row * a.bias_stride + v, left, 0.0f);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float t = x[q][i];
+        const unsigned word = (unsigned)w4[i];
         if constexpr (HIST) {
-          const unsigned c = (unsigned)c4[i] & ~SEEN_IN_PROMPT;
-          if (c4[i] != 0) t = t > 0.0f ? t / rep : t * rep;
-          const float f = freq * (float)c, p = c != 0u ? pres : 0.0f;
-          t = t - (f + p);
+          const unsigned count = SPARSE ? word & COUNT_MASK : word & ~SEEN_IN_PROMPT;
+          const unsigned seen = SPARSE ? word & (SEEN_IN_PROMPT | COUNT_MASK) : word;
+          const float pushed = t > 0.0f ? divide(t, rep, rrep) : t * rep;
+          t = seen != 0u ? pushed : t;
+          t = t - (freq * (float)count + (count != 0u ? pres : 0.0f));
         }
-        if (a.bias != nullptr) t = t + b[q][i];
-        if constexpr (SPARSE) t = t + a4[i];
-        t = (bits[q] >> i & 1u) ? t : NINF;
-        if constexpr (CHOOSE) {
-          float key = t;
-          if (sampled) { t = t * inv; key = t + g[q][i]; }
-          if (!(t == NINF)) {
-            const unsigned long long k = key_of(key, v + i);
-            best = k > best ? k : best;
-          }
-          m = fmaxf(m, t);
+        if (a.bias != nullptr) t = t + b[i];
+        if constexpr (SPARSE) {
+          const unsigned slot = word >> SLOT_SHIFT & SLOT_MASK;
+          if (slot != 0u) t = t + val[slot - 1u];
         }
-        x[q][i] = t;
+        x[q][i] = (now[q] >> i & 1u) ? t : NINF;
       }
       if constexpr (!CHOOSE) {
-        const int left = a.vocab - (int)v;
         O* o = (O*)a.out + row * a.out_stride + v;
         if (left >= 4) Elt<O>::store4(o, x[q]);
         else {
@@ -223,83 +314,109 @@ __global__ void __launch_bounds__(G == 64 ? 256 : G) frl_logits_kernel(const Log
           if (left > 1) o[1] = Elt<O>::put(x[q][1]);
           if (left > 2) o[2] = Elt<O>::put(x[q][2]);
         }
-      }
-    }
-    if constexpr (CHOOSE) {
-      constexpr float LOG2E = 1.4426950408889634f;
-      m = group_reduce<MaxOp, G>(m, red_m);
-      const float m0 = m == NINF ? 0.0f : m;
-      float s = 0.0f;
+      } else {
 #pragma unroll
-      for (int q = 0; q < 2; ++q)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s += __builtin_amdgcn_exp2f((x[q][i] - m0) * LOG2E);
-      best = group_reduce<MaxOp, G>(best, red_k);
-      s = group_reduce<SumOp, G>(s, red_s);
-      // the thread that holds the winner answers; thread 0 where there is none
-      const unsigned win = ~(unsigned)best;
-      bool mine = best == 0 && tid == 0;
-      float y = NINF;
-#pragma unroll
-      for (int q = 0; q < 2; ++q)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (best != 0 && win == v0 + q * 4 * G + 4 * tid + i) { mine = true; y = x[q][i]; }
-      if (mine) {
-        if (a.chunks == 1) {
-          a.token[row] = best != 0 ? (int32_t)win : -1;
-          if (a.logprob != nullptr) a.logprob[row] = best != 0 ? (y - m) - logf(s) : NINF;
-        } else {
-          a.part_key[item] = best;
-          a.part_m[item] = m;
-          a.part_s[item] = s;
-          a.part_y[item] = y;
+        for (int i = 0; i < 4; ++i) {
+          const float y = sampled ? x[q][i] * inv : x[q][i];
+          const float key = sampled ? y + g[q][i] : y;
+          const bool better = key > ch.key;                 // the first of equal keys stays; against a NaN nothing is better
+          ch.key = better ? key : ch.key;
+          ch.y = better ? y : ch.y;
+          ch.v = better ? v + i : ch.v;
+          bm = fmaxf(bm, y);
+          x[q][i] = y;
         }
       }
-      if constexpr (G > 64) __syncthreads();                 // the next item writes red_* again
+      __builtin_amdgcn_sched_barrier(0);                    // one quad at a time: 64 registers let two workgroups of 1024 share a CU
+    }
+    if constexpr (CHOOSE) {
+      if (bm > ch.m) {
+        if (ch.m != NINF) ch.s *= Shift(bm, LOG2E).from(Shift(ch.m, LOG2E));
+        ch.m = bm;
+      }
+      const Shift sh(ch.m == NINF ? 0.0f : ch.m, LOG2E);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        float e[4] = {x[q][0], x[q][1], x[q][2], x[q][3]};
+        sh.exps<4>(e);
+        const float sum = (e[0] + e[1]) + (e[2] + e[3]);
+        ch.s += sum;
+        if (sum != sum && !ch.nan) {                        // a NaN among the four, or infinity less infinity
+#pragma unroll
+          for (int i = 3; i >= 0; --i)
+            if (x[q][i] != x[q][i]) { ch.nan = true; ch.v = v0 + q * 4 * G + 4 * t0 + i; ch.key = ch.y = x[q][i]; }
+        }
+      }
+    }
+  }
+  if constexpr (CHOOSE) {
+    const float m = group_reduce<MaxOp, G>(ch.m, red_m);
+    if (ch.m != NINF) ch.s *= Shift(m, LOG2E).from(Shift(ch.m, LOG2E));
+    unsigned long long best = ch.v != 0xffffffffu ? key_of(ch.key, ch.v) : 0ull;
+    best = group_reduce<MaxOp, G>(best, red_k);
+    const float s = group_reduce<SumOp, G>(ch.s, red_s);
+    const bool none = best == 0;
+    if (none ? tid == 0 : ch.v == ~(unsigned)best) {        // the thread that holds the winner answers
+      if (a.parts == 1) answer(a, row, best, m, s, ch.y);
+      else {
+        a.part_key[item] = best;
+        a.part_m[item] = m;
+        a.part_s[item] = s;
+        a.part_y[item] = ch.y;
+      }
     }
   }
 }
 
-// the chunks of a row joined: one wave per row, a fixed order
+// the parts of a row joined: one wave per row, a fixed order
 __global__ void __launch_bounds__(256) frl_logits_join_kernel(const LogitsArgs a, long long rows) {
-  constexpr float LOG2E = 1.4426950408889634f;
   const int lane = threadIdx.x & 63;
-  for (long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); row < rows; row += (long long)gridDim.x * 4) {
-    const long long at = row * a.chunks;
-    unsigned long long best = 0;
-    float m = -INFINITY, y = -INFINITY;
-    for (unsigned c = lane; c < a.chunks; c += 64) {
-      const unsigned long long k = a.part_key[at + c];
-      if (k > best) { best = k; y = a.part_y[at + c]; }
-      m = fmaxf(m, a.part_m[at + c]);
-    }
-    m = wave_reduce<MaxOp>(m);
-    const float m0 = m == -INFINITY ? 0.0f : m;
-    float s = 0.0f;
-    for (unsigned c = lane; c < a.chunks; c += 64) s += a.part_s[at + c] * __builtin_amdgcn_exp2f((a.part_m[at + c] - m0) * LOG2E);
-    s = wave_reduce<SumOp>(s);
-    const unsigned long long all = wave_reduce<MaxOp>(best);
-    if (all == 0 ? lane == 0 : best == all) {                // indices differ between chunks, so one lane holds the winner
-      a.token[row] = all != 0 ? (int32_t) ~(unsigned)all : -1;
-      if (a.logprob != nullptr) a.logprob[row] = all != 0 ? (y - m) - logf(s) : -INFINITY;
-    }
+  const long long row = block_index() * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const long long at = row * a.parts;
+  unsigned long long best = 0;
+  float m = -INFINITY, y = -INFINITY;
+  for (int c = lane; c < a.parts; c += 64) {
+    const unsigned long long k = a.part_key[at + c];
+    if (k > best) { best = k; y = a.part_y[at + c]; }
+    m = fmaxf(m, a.part_m[at + c]);
   }
+  m = wave_reduce<MaxOp>(m);
+  const Shift sh(m, LOG2E);
+  float s = 0.0f;
+  for (int c = lane; c < a.parts; c += 64) {
+    const float mc = a.part_m[at + c];
+    s += a.part_s[at + c] * (mc == -INFINITY ? 1.0f : sh.from(Shift(mc, LOG2E)));      // a part of -inf alone has a sum of 0 (or NaN)
+  }
+  s = wave_reduce<SumOp>(s);
+  const unsigned long long all = wave_reduce<MaxOp>(best);
+  if (all == 0 ? lane == 0 : best == all) answer(a, row, all, m, s, y);                // indices differ between parts, so one lane holds the winner
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
 
-// Threads per (row, chunk).
-static int logits_group(long long rows, int vocab) {
-  if (vocab <= 512) return 64;
-  const long long wide = rows * ((vocab + 8191) / 8192);
-  return (vocab > 4096 && wide >= 512) ? 1024 : 256;
+struct LogitsPlan { int G, chunks, per, parts; };
+
+// Threads per chunk: a wave for short rows; a workgroup of 1024 where that gives every CU two of them (the history is then searched for the fewest
+// chunks); else 256, which spreads a few rows over more CUs.  A group takes so many chunks of a row that about two rounds of resident groups remain.
+static LogitsPlan logits_plan(const FrlLogitsDesc* d) {
+  LogitsPlan p;
+  const long long wide = d->rows * (((long long)d->vocab + 8191) / 8192);
+  p.G = d->vocab <= 512 && d->n_sparse <= 512 ? 64 : (d->vocab > 4096 && wide >= 512) ? 1024 : 256;
+  p.chunks = (int)((d->vocab + 8LL * p.G - 1) / (8 * p.G));
+  const long long rounds = d->rows * p.chunks / (p.G == 1024 ? 1024 : 4096);
+  p.per = rounds < 1 ? 1 : rounds > p.chunks ? p.chunks : (int)rounds;
+  p.parts = (p.chunks + p.per - 1) / p.per;
+  p.per = (p.chunks + p.parts - 1) / p.parts;
+  return p;
 }
 
 template <typename T, typename O, bool CHOOSE>
-static hipError_t launch_logits(const LogitsArgs& a, int G, unsigned grid, hipStream_t stream) {
+static hipError_t launch_logits(const LogitsArgs& a, int G, hipStream_t stream) {
+  const dim3 grid = grid_of(G == 64 ? (a.items + 3) / 4 : a.items);
+  const size_t lds = (size_t)(G == 64 ? 4 : 1) * a.K * 8;
 #define FRL_LAUNCH(g, h, s)                                                                                             \
-  hipLaunchKernelGGL((frl_logits_kernel<T, O, g, h, s, CHOOSE>), dim3(grid), dim3(g == 64 ? 256 : g), 0, stream, a)
+  hipLaunchKernelGGL((frl_logits_kernel<T, O, g, h, s, CHOOSE>), grid, dim3(g == 64 ? 256 : g), lds, stream, a)
 #define FRL_PICK(g)                                                                                                     \
   do {                                                                                                                  \
     if (a.L > 0 && a.K > 0) FRL_LAUNCH(g, true, true);                                                                  \
@@ -326,16 +443,15 @@ static int logits_validate(const FrlLogitsDesc* d, bool choose) {
   if (d->n_sparse > FRL_LOGITS_MAX_SPARSE) { set_error("logits: %d listed biases per row > %d (use the dense bias)", d->n_sparse, FRL_LOGITS_MAX_SPARSE); return FRL_EUNSUPPORTED; }
   if (d->mask < FRL_MASK_NONE || d->mask > FRL_MASK_BYTES) { set_error("logits: mask %d invalid", d->mask); return FRL_EINVAL; }
   if (d->vocab > (1 << 30)) { set_error("logits: vocab %d > 2^30", d->vocab); return FRL_EUNSUPPORTED; }
-  const int G = logits_group(d->rows, d->vocab);
-  const long long chunks = ((long long)d->vocab + 8 * G - 1) / (8 * G);
-  if (d->rows > (1LL << 30) / chunks) { set_error("logits: %lld rows of %d entries are more than 2^30 chunks in one call", (long long)d->rows, d->vocab); return FRL_EUNSUPPORTED; }
+  if (d->n_sparse > 0 && d->history_len > MAX_HISTORY_WITH_SLOTS) { set_error("logits: history_len %d > %d beside listed biases", d->history_len, MAX_HISTORY_WITH_SLOTS); return FRL_EUNSUPPORTED; }
+  if (d->rows > (1LL << 35) || d->rows * logits_plan(d).chunks > (1LL << 35)) { set_error("logits: %lld rows of %d entries are more than 2^35 chunks in one call", (long long)d->rows, d->vocab); return FRL_EUNSUPPORTED; }
   const long long V = d->vocab;
   if (d->rows > 1 && d->logits_stride < V) { set_error("logits: row stride %lld < vocab %lld", (long long)d->logits_stride, V); return FRL_EINVAL; }
   if (d->rows > 1 && !choose && d->out_stride < V) { set_error("logits: out row stride %lld < vocab %lld", (long long)d->out_stride, V); return FRL_EINVAL; }
   return FRL_OK;
 }
 
-static int logits_fill(const FrlLogitsDesc* d, const FrlLogitsBufs* b, bool choose, LogitsArgs& a, int& G) {
+static int logits_fill(const FrlLogitsDesc* d, const FrlLogitsBufs* b, LogitsArgs& a, int& G) {
   if (b == nullptr || b->logits == nullptr) { set_error("logits: bufs.logits is NULL"); return FRL_EINVAL; }
   if (d->history_len > 0 && b->history == nullptr) { set_error("logits: bufs.history is NULL (history_len %d)", d->history_len); return FRL_EINVAL; }
   if (d->n_sparse > 0 && (b->bias_tokens == nullptr || b->bias_values == nullptr)) { set_error("logits: bufs.bias_tokens / bias_values is NULL (n_sparse %d)", d->n_sparse); return FRL_EINVAL; }
@@ -345,24 +461,17 @@ static int logits_fill(const FrlLogitsDesc* d, const FrlLogitsBufs* b, bool choo
                  b->bias, b->bias_tokens, b->bias_values, b->allowed, b->temperature, b->gumbel, b->token, b->logprob,
                  nullptr, nullptr, nullptr, nullptr,
                  d->logits_stride, d->out_stride, d->gumbel_stride, d->history_stride, d->bias_stride, d->sparse_stride, d->mask_stride,
-                 d->repetition, d->frequency, d->presence, d->temperature, 0, 0, d->vocab, d->ids64, d->history_len, d->n_sparse, d->mask};
-  G = logits_group(d->rows, d->vocab);
-  a.chunks = (unsigned)((d->vocab + 8LL * G - 1) / (8 * G));
-  a.items = (unsigned)(d->rows * a.chunks);
+                 d->repetition, d->frequency, d->presence, d->temperature, d->vocab, d->ids64, d->history_len, d->n_sparse, d->mask, 0, 0, 0, 0};
+  const LogitsPlan p = logits_plan(d);
+  G = p.G;
+  a.chunks = p.chunks; a.per = p.per; a.parts = p.parts;
+  a.items = (long long)d->rows * p.parts;
   return FRL_OK;
 }
 
-// Enough workgroups for every CU to be full many times over; beyond that a workgroup takes several items.
-static unsigned logits_grid(const LogitsArgs& a, int G) {
-  const unsigned groups = G == 64 ? (a.items + 3) / 4 : a.items;
-  return groups < (1u << 20) ? groups : (1u << 20);
-}
-
 static size_t logits_workspace(const FrlLogitsDesc* d) {
-  const int G = logits_group(d->rows, d->vocab);
-  const size_t chunks = (size_t)((d->vocab + 8LL * G - 1) / (8 * G));
-  const size_t items = chunks > 1 ? (size_t)d->rows * chunks : 0;
-  return (items * 20 + 511) / 256 * 256;
+  const int parts = logits_plan(d).parts;
+  return ((parts > 1 ? (size_t)d->rows * parts * 20 : 0) + 511) / 256 * 256;
 }
 
 }  // namespace frl
@@ -378,7 +487,7 @@ int frl_logits_constrain(const FrlLogitsDesc* desc, const FrlLogitsBufs* bufs, v
   if (desc->rows == 0) return FRL_OK;
   LogitsArgs a;
   int G;
-  if ((rc = logits_fill(desc, bufs, false, a, G)) != FRL_OK) return rc;
+  if ((rc = logits_fill(desc, bufs, a, G)) != FRL_OK) return rc;
   if (a.out == nullptr) { set_error("logits: bufs.out is NULL"); return FRL_EINVAL; }
   // in place is the very same rows; any other overlap would be read after it was written
   const size_t in_elt = desc->dtype == FRL_ELT_F32 ? 4 : 2, out_elt = desc->out_dtype == FRL_ELT_F32 ? 4 : 2;
@@ -386,15 +495,14 @@ int frl_logits_constrain(const FrlLogitsDesc* desc, const FrlLogitsBufs* bufs, v
   const uintptr_t o0 = (uintptr_t)a.out, o1 = o0 + ((size_t)(desc->rows - 1) * desc->out_stride + desc->vocab) * out_elt;
   const bool same = i0 == o0 && desc->dtype == desc->out_dtype && (desc->logits_stride == desc->out_stride || desc->rows == 1);
   if (!same && i0 < o1 && o0 < i1) { set_error("logits: out overlaps logits without being the same rows"); return FRL_EINVAL; }
-  const unsigned grid = logits_grid(a, G);
   const bool f32 = desc->out_dtype == FRL_ELT_F32;
   hipStream_t st = (hipStream_t)hip_stream;
   hipError_t e = hipErrorInvalidValue;
-  if (desc->dtype == FRL_ELT_F32) e = launch_logits<float, float, false>(a, G, grid, st);
-  else if (desc->dtype == FRL_ELT_BF16) e = f32 ? launch_logits<Bf16, float, false>(a, G, grid, st) : launch_logits<Bf16, Bf16, false>(a, G, grid, st);
-  else e = f32 ? launch_logits<F16, float, false>(a, G, grid, st) : launch_logits<F16, F16, false>(a, G, grid, st);
+  if (desc->dtype == FRL_ELT_F32) e = launch_logits<float, float, false>(a, G, st);
+  else if (desc->dtype == FRL_ELT_BF16) e = f32 ? launch_logits<Bf16, float, false>(a, G, st) : launch_logits<Bf16, Bf16, false>(a, G, st);
+  else e = f32 ? launch_logits<F16, float, false>(a, G, st) : launch_logits<F16, F16, false>(a, G, st);
   if (e != hipSuccess) { set_error("logits constrain launch: %s", hipGetErrorString(e)); return FRL_EHIP; }
-  note_kernel("frl_logits_kernel<constrain, %d threads> [%u]", G, grid);
+  note_kernel("frl_logits_kernel<constrain, %d threads> [%lld]", G, a.items);
   return FRL_OK;
 }
 
@@ -409,11 +517,11 @@ int frl_logits_choose(const FrlLogitsDesc* desc, const FrlLogitsBufs* bufs, void
   if (desc->rows == 0) return FRL_OK;
   LogitsArgs a;
   int G;
-  if ((rc = logits_fill(desc, bufs, true, a, G)) != FRL_OK) return rc;
+  if ((rc = logits_fill(desc, bufs, a, G)) != FRL_OK) return rc;
   if (a.token == nullptr) { set_error("logits: bufs.token is NULL"); return FRL_EINVAL; }
   if (a.gumbel != nullptr && desc->rows > 1 && desc->gumbel_stride < desc->vocab) { set_error("logits: gumbel row stride %lld < vocab %d", (long long)desc->gumbel_stride, desc->vocab); return FRL_EINVAL; }
   if (a.gumbel == nullptr && a.temperature == nullptr && desc->temperature > 0.0f) { set_error("logits: temperature %g > 0 draws: bufs.gumbel is NULL", desc->temperature); return FRL_EINVAL; }
-  if (a.chunks > 1) {
+  if (a.parts > 1) {
     if (workspace == nullptr || ((uintptr_t)workspace & 255) != 0) { set_error("workspace must be non-NULL and 256-byte aligned"); return FRL_EWORKSPACE; }
     if (workspace_bytes < logits_workspace(desc)) { set_error("workspace %zu B < required %zu B", workspace_bytes, logits_workspace(desc)); return FRL_EWORKSPACE; }
     a.part_key = (unsigned long long*)workspace;
@@ -421,19 +529,17 @@ int frl_logits_choose(const FrlLogitsDesc* desc, const FrlLogitsBufs* bufs, void
     a.part_s = a.part_m + a.items;
     a.part_y = a.part_s + a.items;
   }
-  const unsigned grid = logits_grid(a, G);
   hipStream_t st = (hipStream_t)hip_stream;
-  hipError_t e = desc->dtype == FRL_ELT_F32 ? launch_logits<float, float, true>(a, G, grid, st)
-               : desc->dtype == FRL_ELT_BF16 ? launch_logits<Bf16, float, true>(a, G, grid, st) : launch_logits<F16, float, true>(a, G, grid, st);
+  hipError_t e = desc->dtype == FRL_ELT_F32 ? launch_logits<float, float, true>(a, G, st)
+               : desc->dtype == FRL_ELT_BF16 ? launch_logits<Bf16, float, true>(a, G, st) : launch_logits<F16, float, true>(a, G, st);
   if (e != hipSuccess) { set_error("logits choose launch: %s", hipGetErrorString(e)); return FRL_EHIP; }
-  note_kernel("frl_logits_kernel<choose, %d threads> [%u]", G, grid);
-  if (a.chunks > 1) {
+  note_kernel("frl_logits_kernel<choose, %d threads> [%lld]", G, a.items);
+  if (a.parts > 1) {
     const long long blocks = (desc->rows + 3) / 4;
-    const unsigned jg = (unsigned)(blocks < 65536 ? blocks : 65536);
-    hipLaunchKernelGGL(frl_logits_join_kernel, dim3(jg), dim3(256), 0, st, a, (long long)desc->rows);
+    hipLaunchKernelGGL(frl_logits_join_kernel, grid_of(blocks), dim3(256), 0, st, a, (long long)desc->rows);
     e = hipGetLastError();
     if (e != hipSuccess) { set_error("logits join launch: %s", hipGetErrorString(e)); return FRL_EHIP; }
-    note_kernel("frl_logits_join_kernel [%u]", jg);
+    note_kernel("frl_logits_join_kernel [%lld]", blocks);
   }
   return FRL_OK;
 }
