@@ -21,6 +21,7 @@ struct DistillArgs {
   float* rowloss;             // (rows,) weight * L
   float* stats;               // (rows + 1, 4) or NULL: m, 1 / s, factor of the named entries, factor of the others; last row: 1 / denominator
   const float* inv_denom;     // device 1 / sum of weights, or NULL: `denom_scale`
+  int sum_weights;            // row kernel: every group sums the weights itself
   const float* g_loss;        // backward: cotangent, `g_stride` apart per row (0: one scalar); NULL: 1
   void* grad;
   float* part;                // split rows: (rows, segs, 3) m, s, r
@@ -51,12 +52,6 @@ __device__ __forceinline__ void mark_named(const DistillArgs& a, long long row, 
   group_sync<G>();
 }
 
-template <int N>
-__device__ __forceinline__ float max_of(const float* x, float m) {
-#pragma unroll
-  for (int i = 0; i < N; i += 2) m = fmaxf(fmaxf(x[i], x[i + 1]), m);      // v_max3_f32
-  return m;
-}
 template <int N>
 __device__ __forceinline__ float sum_of(const float* e) {
   float s = 0.0f;
@@ -133,34 +128,36 @@ struct Running {
   }
 };
 
-// What one wave makes of a row's teacher entries: p (into sp, 0 for padding), the tokens (into sid, -1 for padding) and their logits
-// (into sz), sum p and sum p (log p - z / T).  FRL_DISTILL_REST needs 1 - sum p, which float32 exponentials would leave without digits: float64.
-template <typename T, bool REST>
+// What W lanes make of a row's teacher entries: the tokens (into sid, -1 for padding), p (into sp, 0 for padding) and their logits (into sz),
+// sum p and sum p (log p - z / T).  The three loads of an entry are under way together; what follows works on LDS.  FRL_DISTILL_REST needs
+// 1 - sum p, which float32 exponentials would leave without digits: float64.
+template <typename T, int W, bool REST>
 __device__ __forceinline__ void teacher_part(const DistillArgs& a, long long row, const T* z, int lane, int* sid, float* sp, float* sz, double& sum_p, double& cross) {
   sum_p = cross = 0.0;
   float tm = -INFINITY, tot = 0.0f;
+  const void* ids = (const char*)a.ids + row * a.ids_stride * (a.ids64 ? 8 : 4);
+  for (int k = lane; k < a.top; k += W) {
+    const long long id = ld_id(ids, k, a.ids64);
+    const float t = teacher_at(a.teacher, row * a.teacher_stride + k, a.teacher_dtype);
+    const bool valid = id >= 0 && id < a.vocab;
+    sid[k] = valid ? (int)id : -1;
+    sp[k] = t;
+    sz[k] = valid ? Elt<T>::get(z[id]) : 0.0f;
+    if (valid) tm = fmaxf(tm, t);
+  }
   if constexpr (!REST) {
-    for (int k = lane; k < a.top; k += 64) {
-      const long long id = ld_id(a.ids, row * a.ids_stride + k, a.ids64);
-      if (id >= 0 && id < a.vocab) tm = fmaxf(tm, teacher_at(a.teacher, row * a.teacher_stride + k, a.teacher_dtype));
-    }
-    tm = wave_reduce<MaxOp>(tm);
+    tm = lanes_reduce<MaxOp, W>(tm);
     const float t0 = tm == -INFINITY ? 0.0f : tm;
-    for (int k = lane; k < a.top; k += 64) {
-      const long long id = ld_id(a.ids, row * a.ids_stride + k, a.ids64);
-      if (id >= 0 && id < a.vocab) tot += expf((teacher_at(a.teacher, row * a.teacher_stride + k, a.teacher_dtype) - t0) * a.inv_temp);
-    }
-    tot = wave_reduce<SumOp>(tot);
+    for (int k = lane; k < a.top; k += W)
+      if (sid[k] >= 0) tot += expf((sp[k] - t0) * a.inv_temp);
+    tot = lanes_reduce<SumOp, W>(tot);
   }
   const float log_tot = REST ? 0.0f : logf(tot);
-  for (int k = lane; k < a.top; k += 64) {
-    const long long id = ld_id(a.ids, row * a.ids_stride + k, a.ids64);
-    const bool valid = id >= 0 && id < a.vocab;
-    float p = 0.0f, zk = 0.0f;
-    if (valid) {
-      const float t = teacher_at(a.teacher, row * a.teacher_stride + k, a.teacher_dtype);
-      zk = Elt<T>::get(z[id]);
-      const double y = (double)zk * (double)a.scale2 * LN2;      // with the rounded log2(e) / T of the exponentials: one temperature throughout
+  for (int k = lane; k < a.top; k += W) {
+    float p = 0.0f;
+    if (sid[k] >= 0) {
+      const float t = sp[k];
+      const double y = (double)sz[k] * (double)a.scale2 * LN2;   // with the rounded log2(e) / T of the exponentials: one temperature throughout
       float lp;
       if constexpr (REST) {
         const double pd = exp((double)t);
@@ -175,13 +172,13 @@ __device__ __forceinline__ void teacher_part(const DistillArgs& a, long long row
       }
       if (p != 0.0f) cross += (double)p * ((double)lp - y);
     }
-    sid[k] = valid ? (int)id : -1;
     sp[k] = p;
-    sz[k] = zk;
   }
-  sum_p = wave_reduce<SumOp>(sum_p);
-  cross = wave_reduce<SumOp>(cross);
+  sum_p = lanes_reduce<SumOp, W>(sum_p);
+  cross = lanes_reduce<SumOp, W>(cross);
 }
+
+__device__ __forceinline__ float inverse(double s) { return s != 0.0 ? (float)(1.0 / s) : 0.0f; }
 
 struct Factors { float inv_s, k_named, k_rest; };
 
@@ -294,18 +291,19 @@ __device__ __forceinline__ void keep_packed(u32x4* raw) {
 
 // A row to a group, its first NV vectors per thread held in registers: value, what the backward needs, and (GRAD) the gradient.
 template <typename T, int G, int NV, bool REST, bool GRAD>
-__global__ void __launch_bounds__(G == 64 ? 256 : G, 4) frl_distill_row_kernel(const DistillArgs a) {
+__global__ void __launch_bounds__(G <= 64 ? 256 : G, 4) frl_distill_row_kernel(const DistillArgs a) {
   extern __shared__ __align__(16) unsigned lds[];
-  constexpr int GPB = G == 64 ? 4 : 1, N = Vec16<T>::N;
-  __shared__ float red0[G / 64], red1[G / 64];
-  __shared__ double row_p[GPB], row_x[GPB];
-  const int tid = threadIdx.x % G, grp = G == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+  constexpr int GPB = G <= 64 ? 256 / G : 1, N = Vec16<T>::N;
+  constexpr int WAVES = G < 64 ? 1 : G / 64;
+  __shared__ float red0[WAVES], red1[WAVES];
+  __shared__ double row_p[GPB], row_x[GPB], red2[WAVES];
+  const int tid = threadIdx.x % G, grp = G < 64 ? threadIdx.x / G : G == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
   const int nwords = REST ? (a.vocab + 31) / 32 : 0;
   unsigned* words = lds + (size_t)grp * (nwords + 3 * a.top);
   int* sid = (int*)(words + nwords);
   float* sp = (float*)(sid + a.top);
   float* sz = sp + a.top;
-  const float inv = a.inv_denom != nullptr ? *a.inv_denom : a.denom_scale;
+  float inv = a.inv_denom != nullptr ? *a.inv_denom : a.denom_scale;
   const int nvec = a.vocab / N, tail = a.vocab - nvec * N, nv = (nvec + G - 1) / G;
   const long long row = block_index() * GPB + grp;
   if (row >= a.rows) return;
@@ -320,13 +318,7 @@ __global__ void __launch_bounds__(G == 64 ? 256 : G, 4) frl_distill_row_kernel(c
     if constexpr (GRAD) zero_row<T, G>(g, a.vocab, tid);
     return;
   }
-  // the teacher's part first: its float64 temporaries and the row's vectors together would not fit 128 registers
-  if constexpr (REST) mark_named<G>(a, row, tid, 0, a.vocab, words);
-  if (tid < 64) {
-    double sum_p, cross;
-    teacher_part<T, REST>(a, row, z, tid, sid, sp, sz, sum_p, cross);
-    if (tid == 0) { row_p[grp] = sum_p; row_x[grp] = cross; }
-  }
+  // what the row holds is asked for before anything else; the teacher's part works meanwhile
   constexpr int R = NV > 0 ? NV : 1;
   u32x4 raw[R];
   const int t0 = fresh(tid);
@@ -334,6 +326,17 @@ __global__ void __launch_bounds__(G == 64 ? 256 : G, 4) frl_distill_row_kernel(c
   for (int i = 0; i < NV; ++i) {
     raw[i] = Vec16<T>::fill_minus_inf();
     if (i < nv && i * G + t0 < nvec) raw[i] = ldu<u32x4>((const char*)z + 16u * (unsigned)(i * G + t0));
+  }
+  if constexpr (REST) mark_named<G>(a, row, tid, 0, a.vocab, words);
+  if (tid < 64) {
+    double sum_p, cross;
+    teacher_part<T, G < 64 ? G : 64, REST>(a, row, z, tid, sid, sp, sz, sum_p, cross);
+    if (tid == 0) { row_p[grp] = sum_p; row_x[grp] = cross; }
+  }
+  if (GRAD && a.sum_weights) {                              // an eighth of the row's bytes at most, out of the cache, while the row is on its way
+    double sw = 0.0;
+    for (long long i = t0; i < a.rows; i += G) sw += (double)a.weights[i];
+    inv = inverse(group_reduce<SumOp, G>(sw, red2));
   }
   Running<REST> run;
   if (nvec > NV * G) run.template stream<T, G>(z, NV * G, nvec, a.scale2, words, t0);
@@ -368,7 +371,7 @@ __global__ void __launch_bounds__(G == 64 ? 256 : G, 4) frl_distill_row_kernel(c
     }
   const float s = group_reduce<SumOp, G>(run.s, red1);
   const float r = REST ? group_reduce<SumOp, G>(run.r, red0) : 0.0f;   // red0: every thread has read the maximum before the barrier in the sum
-  if constexpr (G == 64) group_sync<G>();                    // the teacher's part is visible (a workgroup has passed barriers since)
+  if constexpr (G <= 64) group_sync<G>();                    // the teacher's part is visible (a workgroup has passed barriers since)
   const double sum_p = row_p[grp];
   const Factors k = row_factors<REST>(s, r, sum_p);
   if constexpr (GRAD) {
@@ -424,41 +427,58 @@ __global__ void __launch_bounds__(G) frl_distill_part_kernel(const DistillArgs a
   }
 }
 
-// one wave per row: the segments joined in order, then the teacher's entries
+// One wave per row: the segments joined in order, then the teacher's entries.  A workgroup of 16 waves that holds every row finishes the loss as well.
 template <typename T, bool REST>
-__global__ void __launch_bounds__(64) frl_distill_join_kernel(const DistillArgs a) {
+__global__ void __launch_bounds__(1024) frl_distill_join_kernel(const DistillArgs a, float* loss, float* inv_out) {
   extern __shared__ __align__(16) unsigned lds[];
-  int* sid = (int*)lds;
+  __shared__ float row_w[16], row_l[16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  int* sid = (int*)lds + (size_t)wave * 3 * a.top;
   float* sp = (float*)(sid + a.top);
   float* sz = sp + a.top;
-  const int lane = threadIdx.x;
-  const long long row = block_index();
-  if (row >= a.rows) return;
-  const float w = a.weights != nullptr ? a.weights[row] : 1.0f;
-  if (w == 0.0f) {
-    if (lane == 0) {
-      a.rowloss[row] = 0.0f;
-      if (a.stats != nullptr) *(f32x4*)(a.stats + 4 * row) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  const long long row = block_index() * waves + wave;
+  float w = 0.0f, value = 0.0f;
+  if (row < a.rows) {
+    w = a.weights != nullptr ? a.weights[row] : 1.0f;
+    f32x4 st = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (w != 0.0f) {
+      double sum_p, cross;
+      teacher_part<T, 64, REST>(a, row, (const T*)a.logits + row * a.logits_stride, lane, sid, sp, sz, sum_p, cross);
+      float m = -INFINITY, s = 0.0f, r = 0.0f;
+      const float* p = a.part + 3 * row * a.segs;
+      for (int i = lane; i < a.segs; i += 64) m = fmaxf(m, p[3 * i]);
+      m = wave_reduce<MaxOp>(m);
+      for (int i = lane; i < a.segs; i += 64) {
+        const float f = p[3 * i] == -INFINITY ? 1.0f : Shift(m, a.scale2).from(Shift(p[3 * i], a.scale2));     // a segment of -inf alone has sums of 0 (or NaN)
+        s += p[3 * i + 1] * f;
+        r += p[3 * i + 2] * f;
+      }
+      s = wave_reduce<SumOp>(s);
+      r = wave_reduce<SumOp>(r);
+      const Factors k = row_factors<REST>(s, r, sum_p);
+      value = w * row_loss<REST>(a, m, s, r, sum_p, cross);
+      st = f32x4{m, k.inv_s, k.k_named, k.k_rest};
     }
-    return;
+    if (lane == 0) {
+      a.rowloss[row] = value;
+      if (a.stats != nullptr) *(f32x4*)(a.stats + 4 * row) = st;
+    }
   }
-  double sum_p, cross;
-  teacher_part<T, REST>(a, row, (const T*)a.logits + row * a.logits_stride, lane, sid, sp, sz, sum_p, cross);
-  float m = -INFINITY, s = 0.0f, r = 0.0f;
-  const float* p = a.part + 3 * row * a.segs;
-  for (int i = lane; i < a.segs; i += 64) m = fmaxf(m, p[3 * i]);
-  m = wave_reduce<MaxOp>(m);
-  for (int i = lane; i < a.segs; i += 64) {
-    const float f = p[3 * i] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((p[3 * i] - m) * a.scale2);     // a segment of -inf alone has sums of 0 (or NaN)
-    s += p[3 * i + 1] * f;
-    r += p[3 * i + 2] * f;
-  }
-  s = wave_reduce<SumOp>(s);
-  r = wave_reduce<SumOp>(r);
-  const Factors k = row_factors<REST>(s, r, sum_p);
+  if (loss == nullptr) return;
   if (lane == 0) {
-    a.rowloss[row] = w * row_loss<REST>(a, m, s, r, sum_p, cross);
-    if (a.stats != nullptr) *(f32x4*)(a.stats + 4 * row) = f32x4{m, k.inv_s, k.k_named, k.k_rest};
+    row_w[wave] = w;
+    row_l[wave] = value;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double sw = 0.0, sl = 0.0;
+    for (int i = 0; i < waves; ++i) {
+      sw += (double)row_w[i];
+      sl += (double)row_l[i];
+    }
+    const float f = inv_out != nullptr ? inverse(sw) : a.denom_scale;
+    if (inv_out != nullptr) *inv_out = f;
+    *loss = (float)(sl * (double)f);
   }
 }
 
@@ -493,7 +513,7 @@ __global__ void __launch_bounds__(G == 64 ? 256 : G) frl_distill_grad_kernel(con
   if (tid < tail) g[v0 + nvec * N + tid] = Elt<T>::put(sc.one(Elt<T>::get(z[v0 + nvec * N + tid])));
   if (tid < 64) {
     double sum_p, cross;
-    teacher_part<T, REST>(a, row, z, tid, sid, sp, sz, sum_p, cross);
+    teacher_part<T, 64, REST>(a, row, z, tid, sid, sp, sz, sum_p, cross);
   }
   group_sync<G>();
   named_gradient<T, G>(a, g, v0, n, sh, f * st[2] * st[1], f, sid, sp, sz, tid);
@@ -501,51 +521,66 @@ __global__ void __launch_bounds__(G == 64 ? 256 : G) frl_distill_grad_kernel(con
 
 // ---- over the rows ------------------------------------------------------------------------------------------------------
 
-__device__ __forceinline__ double block_sum(double v, double* red) {
-  v = wave_reduce<SumOp>(v);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+// The sum of n floats by one workgroup of 1024 in float64, in a fixed order; thread 0 has it.  One workgroup, because a second one would need a second
+// launch or a counter; eight loads of four floats are under way per thread before the first is added (32768 rows in one go).
+__device__ __forceinline__ double sum_of_rows(const float* __restrict__ x, long long n) {
+  __shared__ double red[16];
+  double s = 0.0;
+  const long long quads = n / 4;
+  for (long long i = threadIdx.x; i < quads; i += 8 * 1024) {
+    f32x4 v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = i + u * 1024 < quads ? ldu<f32x4>(x + 4 * (i + u * 1024)) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int u = 0; u < 8; ++u) s += ((double)v[u][0] + (double)v[u][1]) + ((double)v[u][2] + (double)v[u][3]);
+  }
+  if (threadIdx.x < n - 4 * quads) s += (double)x[4 * quads + threadIdx.x];
+  s = wave_reduce<SumOp>(s);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
-  v = red[0];
-  for (int w = 1; w < (int)(blockDim.x >> 6); ++w) v += red[w];
-  __syncthreads();
-  return v;
+  if (threadIdx.x >= 64) return 0.0;
+  return wave_reduce<SumOp>(threadIdx.x < 16 ? red[threadIdx.x] : 0.0);
 }
 
-// 1 / sum of the weights (0 where the sum is 0), or 1 / rows
+// 1 / sum of the weights, 0 where the sum is 0: ahead of a gradient that is too short to sum them itself
 __global__ void __launch_bounds__(1024) frl_distill_denom_kernel(const float* __restrict__ w, long long rows, float* __restrict__ inv) {
-  __shared__ double red[16];
-  double s = 0.0;
-  for (long long i = threadIdx.x; i < rows; i += 1024) s += (double)w[i];
-  s = block_sum(s, red);
-  if (threadIdx.x == 0) *inv = s != 0.0 ? (float)(1.0 / s) : 0.0f;
+  const double s = sum_of_rows(w, rows);
+  if (threadIdx.x == 0) *inv = inverse(s);
 }
 
-__global__ void __launch_bounds__(1024) frl_distill_sum_kernel(const float* __restrict__ rowloss, long long rows, const float* __restrict__ inv, float scale,
-                                                               float* __restrict__ loss) {
-  __shared__ double red[16];
-  double s = 0.0;
-  for (long long i = threadIdx.x; i < rows; i += 1024) s += (double)rowloss[i];
-  s = block_sum(s, red);
-  if (threadIdx.x == 0) *loss = (float)(s * (double)(inv != nullptr ? *inv : scale));
+// loss = the rows' losses summed, times *inv or scale; with weights their inverse sum is the factor, and is left in inv for the backward
+__global__ void __launch_bounds__(1024) frl_distill_sum_kernel(const float* __restrict__ rowloss, long long rows, const float* __restrict__ w, float* __restrict__ inv,
+                                                               float scale, float* __restrict__ loss) {
+  if (w != nullptr) {
+    const double s = sum_of_rows(w, rows);
+    scale = inverse(s);
+    if (threadIdx.x == 0) *inv = scale;
+    __syncthreads();
+  } else if (inv != nullptr) {
+    scale = *inv;
+  }
+  const double s = sum_of_rows(rowloss, rows);
+  if (threadIdx.x == 0) *loss = (float)(s * (double)scale);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
 
 struct DistillPlan { int G, NV, segs, seg_len; bool split; };
 
-// Threads per row: as few as hold it with 16 vectors of 16 bytes each, more while the rows alone leave the chip's 1024 SIMDs short of four
+// Threads per row: 16 lanes for a row of at most 256 entries and 64 names, else as few as hold it with 16 vectors of 16 bytes each, more while the rows alone leave the chip's 1024 SIMDs short of four
 // waves.  A value alone keeps nothing and streams, up to 1024 threads; a gradient keeps what 512 threads hold (two workgroups to a CU, one
 // loads while the other computes) and reads the rest of a longer row again.  Measured, bf16, value + gradient: 8192 x 131072 990 us so, 1127
 // with 1024 threads and all of it held, 1158 with nothing held; 4096 x 32000 130 with 256 threads, 157 with 512; 2048 x 131072, value alone:
 // 95 us streamed by 1024 threads, 115 held by 512.
 // Fewer than 256 rows of more than 8192 entries, and rows whose named bits would take more than 32 KB of LDS, are split: at least 512 segments,
 // each of 4096 to 65536 entries.
-static DistillPlan distill_plan(long long rows, int vocab, int dtype, bool grad) {
-  const int vec = dtype == FRL_ELT_F32 ? 4 : 8;
-  DistillPlan p = {64, 0, 1, vocab, false};
+static DistillPlan distill_plan(const FrlDistillDesc* d, bool grad) {
+  const long long rows = d->rows;
+  const int vocab = d->vocab, vec = d->dtype == FRL_ELT_F32 ? 4 : 8;
+  DistillPlan p = {vocab <= 256 && d->top <= 64 ? 16 : 64, 0, 1, vocab, false};
   if (vocab <= DROW_MAX && !(rows < 256 && vocab > 8192)) {
     const int most = grad ? 512 : 1024;
-    auto next = [](int G) { return G == 64 ? 256 : 2 * G; };
+    auto next = [](int G) { return G < 256 ? 4 * G : 2 * G; };
     while (p.G < most && vocab > p.G * 16 * vec) p.G = next(p.G);
     while (p.G < most && rows * p.G < 4096 * 64 && vocab > 2 * p.G * vec) p.G = next(p.G);
     if (grad) p.NV = vocab <= p.G * 4 * vec ? 4 : 16;
@@ -613,17 +648,20 @@ static DistillWs distill_ws(const FrlDistillDesc* d, const DistillPlan& p) {
 template <typename T, bool REST>
 static hipError_t launch_rows(const DistillArgs& a, const DistillPlan& p, bool grad, hipStream_t st) {
   const size_t per = ((size_t)(REST ? (a.vocab + 31) / 32 : 0) + 3 * (size_t)a.top) * 4;
-  const size_t lds = p.G == 64 ? 4 * per : per;
-  const long long blocks = p.G == 64 ? (a.rows + 3) / 4 : a.rows;
+  const int gpb = p.G <= 64 ? 256 / p.G : 1;
+  const size_t lds = gpb * per;
+  const long long blocks = (a.rows + gpb - 1) / gpb;
   const dim3 grid = grid_of(blocks);
-#define FRL_GO(g, nv, gr) hipLaunchKernelGGL((frl_distill_row_kernel<T, g, nv, REST, gr>), grid, dim3(g == 64 ? 256 : g), lds, st, a)
+#define FRL_GO(g, nv, gr) hipLaunchKernelGGL((frl_distill_row_kernel<T, g, nv, REST, gr>), grid, dim3(g <= 64 ? 256 : g), lds, st, a)
   if (!grad) {
-    if (p.G == 64) FRL_GO(64, 0, false);
+    if (p.G == 16) FRL_GO(16, 0, false);
+    else if (p.G == 64) FRL_GO(64, 0, false);
     else if (p.G == 256) FRL_GO(256, 0, false);
     else if (p.G == 512) FRL_GO(512, 0, false);
     else FRL_GO(1024, 0, false);
   } else if (p.NV == 4) {
-    if (p.G == 64) FRL_GO(64, 4, true);
+    if (p.G == 16) FRL_GO(16, 4, true);
+    else if (p.G == 64) FRL_GO(64, 4, true);
     else if (p.G == 256) FRL_GO(256, 4, true);
     else FRL_GO(512, 4, true);
   } else {
@@ -636,23 +674,26 @@ static hipError_t launch_rows(const DistillArgs& a, const DistillPlan& p, bool g
   return hipGetLastError();
 }
 
+// `loss` and `inv` (mean over weights): where the join is one workgroup, it finishes them
 template <typename T, bool REST>
-static hipError_t launch_parts(const DistillArgs& a, hipStream_t st) {
+static hipError_t launch_parts(const DistillArgs& a, float* loss, float* inv, hipStream_t st) {
   const long long items = a.rows * a.segs;
   hipLaunchKernelGGL((frl_distill_part_kernel<T, 256, REST>), grid_of(items), dim3(256), REST ? (size_t)((a.seg_len + 31) / 32) * 4 : 0, st, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((frl_distill_join_kernel<T, REST>), grid_of(a.rows), dim3(64), (size_t)a.top * 12, st, a);
-  note_kernel("frl_distill_part_kernel [%lld] + frl_distill_join_kernel [%lld]", items, a.rows);
+  const int waves = loss != nullptr ? (int)a.rows : 1;
+  hipLaunchKernelGGL((frl_distill_join_kernel<T, REST>), grid_of((a.rows + waves - 1) / waves), dim3(64 * waves), (size_t)waves * a.top * 12, st, a, loss, inv);
+  note_kernel("frl_distill_part_kernel [%lld] + frl_distill_join_kernel<%d rows> [%lld]", items, waves, (a.rows + waves - 1) / waves);
   return hipGetLastError();
 }
 
 template <typename T, bool REST>
 static hipError_t launch_grad(const DistillArgs& a, const DistillPlan& p, hipStream_t st) {
-  const long long items = a.rows * a.segs, blocks = p.G == 64 ? (items + 3) / 4 : items;
+  const bool wave = p.G <= 64;
+  const long long items = a.rows * a.segs, blocks = wave ? (items + 3) / 4 : items;
   const dim3 grid = grid_of(blocks);
-  const size_t lds = (size_t)a.top * 12 * (p.G == 64 ? 4 : 1);
-  if (p.G == 64) hipLaunchKernelGGL((frl_distill_grad_kernel<T, 64, REST>), grid, dim3(256), lds, st, a);
+  const size_t lds = (size_t)a.top * 12 * (wave ? 4 : 1);
+  if (wave) hipLaunchKernelGGL((frl_distill_grad_kernel<T, 64, REST>), grid, dim3(256), lds, st, a);
   else if (p.G == 256) hipLaunchKernelGGL((frl_distill_grad_kernel<T, 256, REST>), grid, dim3(256), lds, st, a);
   else hipLaunchKernelGGL((frl_distill_grad_kernel<T, 1024, REST>), grid, dim3(1024), lds, st, a);
   note_kernel("frl_distill_grad_kernel<%d threads> [%lld]", p.G, blocks);
@@ -671,7 +712,7 @@ extern "C" {
 
 size_t frl_distill_workspace_bytes(const FrlDistillDesc* desc) {
   if (distill_validate(desc) != FRL_OK) return 0;
-  return distill_ws(desc, distill_plan(desc->rows, desc->vocab, desc->dtype, true)).total;
+  return distill_ws(desc, distill_plan(desc, true)).total;
 }
 
 int frl_distill_fwd(const FrlDistillDesc* desc, const FrlDistillBufs* bufs, void* workspace, size_t workspace_bytes, void* hip_stream) {
@@ -685,7 +726,7 @@ int frl_distill_fwd(const FrlDistillDesc* desc, const FrlDistillBufs* bufs, void
   const bool grad = bufs->grad != nullptr && desc->rows > 0;
   if (grad && desc->rows > 1 && desc->grad_stride < desc->vocab) { set_error("distill: grad row stride %lld < vocab %d", (long long)desc->grad_stride, desc->vocab); return FRL_EINVAL; }
   if (grad && distill_overlap(desc, bufs)) { set_error("distill: grad overlaps logits"); return FRL_EINVAL; }
-  const DistillPlan p = distill_plan(desc->rows, desc->vocab, desc->dtype, grad);
+  const DistillPlan p = distill_plan(desc, grad);
   const DistillWs w = distill_ws(desc, p);
   if (workspace == nullptr || ((uintptr_t)workspace & 255) != 0) { set_error("workspace must be non-NULL and 256-byte aligned"); return FRL_EWORKSPACE; }
   if (workspace_bytes < w.total) { set_error("workspace %zu B < required %zu B", workspace_bytes, w.total); return FRL_EWORKSPACE; }
@@ -698,25 +739,36 @@ int frl_distill_fwd(const FrlDistillDesc* desc, const FrlDistillBufs* bufs, void
   a.stats = bufs->row_stats != nullptr ? bufs->row_stats : (split && grad) ? ws + w.stats : nullptr;
   a.part = ws + w.part;
   hipError_t e = hipSuccess;
-  if (desc->reduction == FRL_REDUCE_MEAN && bufs->weights != nullptr && desc->rows > 0) {
-    float* inv = bufs->row_stats != nullptr ? bufs->row_stats + 4 * desc->rows : ws + w.inv;
-    a.inv_denom = inv;
-    hipLaunchKernelGGL(frl_distill_denom_kernel, dim3(1), dim3(1024), 0, st, bufs->weights, (long long)desc->rows, inv);
-    e = hipGetLastError();
-    if (e == hipSuccess) note_kernel("frl_distill_denom_kernel");
-  }
-  if (e == hipSuccess && desc->rows > 0) {
-    if (split) {
-      e = FRL_BY_TYPE(launch_parts)(a, st);
-      if (e == hipSuccess && grad) e = FRL_BY_TYPE(launch_grad)(a, p, st);
-    } else {
-      e = FRL_BY_TYPE(launch_rows)(a, p, grad, st);
+  const bool reduce = desc->reduction != FRL_REDUCE_NONE, weighted = desc->reduction == FRL_REDUCE_MEAN && bufs->weights != nullptr && desc->rows > 0;
+  float* inv = weighted ? (bufs->row_stats != nullptr ? bufs->row_stats + 4 * desc->rows : ws + w.inv) : nullptr;
+  // A gradient needs the weights' sum before it starts.  Rows of eight times the weights' bytes sum them
+  // in every group (8192 x 131072 bf16: 940 against 948 + 5 us); at less a kernel of its own does (4096 x 32000: 115 + 5 against 132 us).
+  const size_t elt = desc->dtype == FRL_ELT_F32 ? 4 : 2;
+  const bool finish = split && reduce && desc->rows <= 16 && desc->top * desc->rows * 12 <= 48 * 1024;     // the join is one workgroup and finishes the loss
+  bool have_inv = false;
+  if (weighted && grad && !split) {
+    a.sum_weights = (size_t)desc->rows * 4 * 8 <= (size_t)desc->vocab * elt;
+    if (!a.sum_weights) {
+      hipLaunchKernelGGL(frl_distill_denom_kernel, dim3(1), dim3(1024), 0, st, bufs->weights, (long long)desc->rows, inv);
+      e = hipGetLastError();
+      note_kernel("frl_distill_denom_kernel");
+      have_inv = true;
     }
   }
-  if (e == hipSuccess && desc->reduction != FRL_REDUCE_NONE) {
-    hipLaunchKernelGGL(frl_distill_sum_kernel, dim3(1), dim3(1024), 0, st, a.rowloss, (long long)desc->rows, a.inv_denom, desc->rows > 0 ? a.denom_scale : 0.0f, bufs->loss);
+  a.inv_denom = have_inv ? inv : nullptr;
+  if (e == hipSuccess && desc->rows > 0) {
+    if (split) e = FRL_BY_TYPE(launch_parts)(a, finish ? bufs->loss : nullptr, inv, st);
+    else e = FRL_BY_TYPE(launch_rows)(a, p, grad, st);
+  }
+  if (e == hipSuccess && reduce && !finish) {
+    hipLaunchKernelGGL(frl_distill_sum_kernel, dim3(1), dim3(1024), 0, st, a.rowloss, (long long)desc->rows, weighted && !have_inv ? bufs->weights : nullptr, inv,
+                       desc->rows > 0 ? a.denom_scale : 0.0f, bufs->loss);
     e = hipGetLastError();
-    if (e == hipSuccess) note_kernel("frl_distill_sum_kernel");
+    note_kernel("frl_distill_sum_kernel");
+  }
+  if (e == hipSuccess && split && grad) {
+    a.inv_denom = inv;
+    e = FRL_BY_TYPE(launch_grad)(a, p, st);
   }
   if (e != hipSuccess) { set_error("distill launch: %s", hipGetErrorString(e)); return FRL_EHIP; }
   return FRL_OK;
@@ -732,7 +784,7 @@ int frl_distill_bwd(const FrlDistillDesc* desc, const FrlDistillBufs* bufs, void
   if (((uintptr_t)bufs->row_stats & 15) != 0) { set_error("distill: bufs.row_stats must be 16-byte aligned"); return FRL_EINVAL; }
   if (desc->rows > 1 && desc->grad_stride < desc->vocab) { set_error("distill: grad row stride %lld < vocab %d", (long long)desc->grad_stride, desc->vocab); return FRL_EINVAL; }
   if (distill_overlap(desc, bufs)) { set_error("distill: grad overlaps logits"); return FRL_EINVAL; }
-  const DistillPlan p = distill_plan(desc->rows, desc->vocab, desc->dtype, false);
+  const DistillPlan p = distill_plan(desc, false);
   DistillArgs a = distill_args(desc, bufs, p);
   a.stats = bufs->row_stats;
   a.g_loss = bufs->g_loss;

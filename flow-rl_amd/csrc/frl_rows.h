@@ -2,6 +2,8 @@
 // alignment, reductions over the group of threads that shares a row.  Not part of the public ABI.
 #pragma once
 
+#include <type_traits>
+
 #include "frl_device.h"
 
 // No product is fused into a sum but where the code says so (also for what follows in the including file): results do not depend on
@@ -107,11 +109,11 @@ __device__ __forceinline__ long long ld_id(const void* p, long long i, int ids64
   return ids64 ? ((const long long*)p)[i] : (long long)((const int*)p)[i];
 }
 
-// A group of G threads shares a row: one wave (four groups to a workgroup of 256) or a whole workgroup.  A wave's LDS
-// accesses execute in order, so a one-wave group needs the compiler kept from reordering them and no barrier.
+// A group of G threads shares a row: 16 lanes or one wave (16 or four groups to a workgroup of 256), or a whole workgroup.  A wave's LDS
+// accesses execute in order, so a group within one needs the compiler kept from reordering them and no barrier.
 template <int G>
 __device__ __forceinline__ void group_sync() {
-  if constexpr (G == 64) {
+  if constexpr (G <= 64) {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
     __builtin_amdgcn_wave_barrier();
   } else {
@@ -148,6 +150,13 @@ struct Shift {
   }
 };
 
+template <int N>
+__device__ __forceinline__ float max_of(const float* x, float m) {
+#pragma unroll
+  for (int i = 0; i < N; i += 2) m = fmaxf(fmaxf(x[i], x[i + 1]), m);      // v_max3_f32
+  return m;
+}
+
 // A grid of any number of workgroups: the second dimension takes over where the first times the workgroup would pass 2^32 threads.
 inline dim3 grid_of(long long blocks) {
   const long long x = blocks < (1 << 20) ? blocks : (1 << 20);
@@ -182,22 +191,26 @@ __device__ __forceinline__ unsigned long long lane_of(unsigned long long v, int 
 }
 __device__ __forceinline__ double lane_of(double v, int l) { return __builtin_bit_cast(double, lane_of(__builtin_bit_cast(unsigned long long, v), l)); }
 
-// Over the 64 lanes, all of which have to be active: neighbours, quads and halves of a row of 16 by DPP, then the four rows by lane reads.
+// Over W lanes, all of which have to be active: neighbours, quads and halves of a row of 16 by DPP, then the four rows by lane reads.
 // Every lane gets the result; the order of the operations is fixed.
-template <typename Op, typename V>
-__device__ __forceinline__ V wave_reduce(V v) {
+template <typename Op, int W, typename V>
+__device__ __forceinline__ V lanes_reduce(V v) {
+  static_assert(W == 16 || W == 64, "a row of lanes or a wave");
   v = Op::f(v, dpp<0xB1>(v));      // quad_perm 1 0 3 2
   v = Op::f(v, dpp<0x4E>(v));      // quad_perm 2 3 0 1
   v = Op::f(v, dpp<0x141>(v));     // row_half_mirror: the other quad of eight
   v = Op::f(v, dpp<0x140>(v));     // row_mirror: the other eight of the row
-  return Op::f(Op::f(lane_of(v, 0), lane_of(v, 16)), Op::f(lane_of(v, 32), lane_of(v, 48)));
+  if constexpr (W == 16) return v;
+  else return Op::f(Op::f(lane_of(v, 0), lane_of(v, 16)), Op::f(lane_of(v, 32), lane_of(v, 48)));
 }
+template <typename Op, typename V>
+__device__ __forceinline__ V wave_reduce(V v) { return lanes_reduce<Op, 64>(v); }
 
 // Every thread of the group gets the result; the order of the operations is fixed.  `red` holds one V per wave of the group
 // and is free again after the next group_sync the caller makes (callers alternate between two arrays).
 template <typename Op, int G, typename V>
 __device__ __forceinline__ V group_reduce(V v, V* red) {
-  v = wave_reduce<Op>(v);
+  v = lanes_reduce<Op, G < 64 ? G : 64>(v);
   if constexpr (G > 64) {
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();

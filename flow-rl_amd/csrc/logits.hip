@@ -22,7 +22,7 @@ struct LogitsArgs {
   unsigned long long* part_key; float* part_m; float* part_s; float* part_y;   // choose over several chunks: one entry per (row, chunk)
   long long logits_stride, out_stride, gumbel_stride, history_stride, bias_stride, sparse_stride, mask_stride;
   float rep, freq, pres, temp;
-  int vocab, ids64, L, K, mask;
+  int vocab, ids64, L, K, mask, eager;
   long long items;          // rows x parts
   int chunks, per, parts;   // of a row: chunks of 8 G entries, `per` of them to a part (one group's work)
 };
@@ -113,22 +113,27 @@ __device__ __forceinline__ void stage_listed(const LogitsArgs& a, long long row,
   }
 }
 
-// allowed bits of entries v .. v + 3 (v a multiple of 4, v < vocab); bits beyond the vocabulary are unspecified
-__device__ __forceinline__ unsigned allowed4(const LogitsArgs& a, long long row, unsigned v) {
+// allowed bits of entries v .. v + 3 (v a multiple of 4), of which `left` are in the vocabulary
+template <bool FULL>
+__device__ __forceinline__ unsigned allowed4(const LogitsArgs& a, const void* mask, unsigned v, int left) {
+  if (!FULL && left <= 0) return 0u;
+  unsigned bits = 15u;
   if (a.mask == FRL_MASK_WORDS) {
-    const unsigned w = ((const unsigned*)a.allowed)[row * a.mask_stride + (v >> 5)];
-    return (w >> (v & 31)) & 15u;
+    bits = (((const unsigned*)mask)[v >> 5] >> (v & 31)) & 15u;
+  } else if (a.mask == FRL_MASK_BYTES) {
+    const unsigned char* b = (const unsigned char*)mask + v;
+    if (FULL || left >= 4) {
+      unsigned w = ldu<unsigned>(b);
+      w |= w >> 4;
+      w |= w >> 2;
+      w |= w >> 1;
+      bits = ((w & 0x01010101u) * 0x10204080u) >> 28;       // byte i's lowest bit to bit i
+    } else {
+      bits = 0u;
+      for (int i = 0; i < left; ++i) bits |= (b[i] != 0 ? 1u : 0u) << i;
+    }
   }
-  const unsigned char* b = (const unsigned char*)a.allowed + row * a.mask_stride + v;
-  unsigned bits = 0;
-  if ((int)v + 4 <= a.vocab) {
-    const unsigned w = ldu<unsigned>(b);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) bits |= ((w >> (8 * i) & 255u) != 0u ? 1u : 0u) << i;
-  } else {
-    for (int i = 0; (int)v + i < a.vocab; ++i) bits |= (b[i] != 0 ? 1u : 0u) << i;
-  }
-  return bits;
+  return FULL || left >= 4 ? bits : bits & ((1u << left) - 1u);
 }
 
 template <typename T>
@@ -208,11 +213,11 @@ __global__ void __launch_bounds__(G == 64 ? 256 : G, 8) frl_logits_kernel(const 
   const float inv = sampled ? 1.0f / (1e-6f + temp) : 1.0f;
   const float* noise = sampled ? a.gumbel + row * a.gumbel_stride : nullptr;
 
+  const void* mask = a.mask == FRL_MASK_WORDS ? (const void*)((const unsigned*)a.allowed + row * a.mask_stride) : (const void*)((const unsigned char*)a.allowed + row * a.mask_stride);
+  const int whole = a.vocab / CH;                           // chunks before this one lie in the vocabulary altogether
   auto bits_of = [&](int c, int q, int t) -> unsigned {
-    const int v = c * CH + q * 4 * G + 4 * t, left = a.vocab - v;
-    if (left <= 0 || c >= c1) return 0u;
-    unsigned b = a.mask != FRL_MASK_NONE ? allowed4(a, row, v) : 15u;
-    return left < 4 ? b & ((1u << left) - 1u) : b;
+    const unsigned v = (unsigned)c * CH + q * 4 * G + 4 * t;
+    return c >= c1 ? 0u : c < whole ? allowed4<true>(a, mask, v, 4) : allowed4<false>(a, mask, v, a.vocab - (int)v);
   };
   unsigned bits[2] = {bits_of(c0, 0, tid), bits_of(c0, 1, tid)};
 
@@ -239,28 +244,29 @@ __global__ void __launch_bounds__(G == 64 ? 256 : G, 8) frl_logits_kernel(const 
   }
 
   Choice ch;
-  for (int c = c0; c < c1; ++c) {
+  float ahead = NINF;                                       // the best key that any lane of the wave has
+  auto chunk = [&](int c, auto full) {
+    constexpr bool FULL = decltype(full)::value;
     const int t0 = fresh(tid);
-    const unsigned v0 = (unsigned)c * CH, n = min((unsigned)a.vocab - v0, (unsigned)CH);
+    const unsigned v0 = (unsigned)c * CH, n = FULL ? (unsigned)CH : (unsigned)a.vocab - v0;
     Packed4<T> raw[2];
     f32x4 g[2];
-    // everything that streams is asked for first; a quad of which nothing is allowed is not read at all
+    // everything that streams is asked for first.  In a batch that fills the chip a quad of which nothing is allowed is not read at all; a small one
+    // does not wait for its mask
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       const unsigned v = v0 + q * 4 * G + 4 * t0;
-      const int left = a.vocab - (int)v;
+      const int left = FULL ? 4 : a.vocab - (int)v;
       raw[q].none();
       g[q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      if (bits[q] != 0u) {
-        raw[q].load(z + v, left);
-        if (sampled) g[q] = load_quad(noise + v, left, 0.0f);
+      if (a.eager ? left > 0 : bits[q] != 0u) {
+        raw[q].load((const T*)((const char*)z + v * (unsigned)sizeof(T)), left);
+        if (sampled) g[q] = load_quad((const float*)((const char*)noise + v * 4u), left, 0.0f);
       }
     }
     const unsigned now[2] = {bits[0], bits[1]};
-    if (a.mask != FRL_MASK_NONE || c + 2 >= c1) {
-      bits[0] = bits_of(c + 1, 0, t0);
-      bits[1] = bits_of(c + 1, 1, t0);
-    }
+    bits[0] = bits_of(c + 1, 0, t0);
+    bits[1] = bits_of(c + 1, 1, t0);
     unsigned* w = cnt + (WORDS ? ((c - c0) & 1) * CH : 0);
     if constexpr (HIST) {
 #pragma unroll
@@ -273,14 +279,13 @@ __global__ void __launch_bounds__(G == 64 ? 256 : G, 8) frl_logits_kernel(const 
         if (loc < n) atomicAdd(&w[loc], (unsigned)(k + 1) << SLOT_SHIFT);
       }
     }
-    f32x4 x[2];
-    float bm = ch.m;
+    float x[2][4], top[2];
     if constexpr (WORDS) group_sync<G>();                   // the words are complete; the other set was cleared by the threads that read it
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       const unsigned v = v0 + q * 4 * G + 4 * t0;
-      const int left = a.vocab - (int)v;
-      x[q] = raw[q].get();
+      const int left = FULL ? 4 : a.vocab - (int)v;
+      const f32x4 in = raw[q].get();
       i32x4 w4 = {0, 0, 0, 0};
       if constexpr (WORDS) {
         w4 = *(const i32x4*)(w + q * 4 * G + 4 * t0);
@@ -290,9 +295,9 @@ __global__ void __launch_bounds__(G == 64 ? 256 : G, 8) frl_logits_kernel(const 
       if (a.bias != nullptr && now[q] != 0u) b = load_quad(a.bias + row * a.bias_stride + v, left, 0.0f);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float t = x[q][i];
+        float t = in[i];
         const unsigned word = (unsigned)w4[i];
-        if constexpr (HIST) {
+        if (HIST && word != 0u) {                           // few tokens are listed: often no lane of a wave has one, and the wave skips this
           const unsigned count = SPARSE ? word & COUNT_MASK : word & ~SEEN_IN_PROMPT;
           const unsigned seen = SPARSE ? word & (SEEN_IN_PROMPT | COUNT_MASK) : word;
           const float pushed = t > 0.0f ? divide(t, rep, rrep) : t * rep;
@@ -304,37 +309,49 @@ __global__ void __launch_bounds__(G == 64 ? 256 : G, 8) frl_logits_kernel(const 
           const unsigned slot = word >> SLOT_SHIFT & SLOT_MASK;
           if (slot != 0u) t = t + val[slot - 1u];
         }
-        x[q][i] = (now[q] >> i & 1u) ? t : NINF;
+        const unsigned keep = (unsigned)((int)(now[q] << (31 - i)) >> 31);
+        x[q][i] = __uint_as_float((__float_as_uint(t) & keep) | (0xff800000u & ~keep));
       }
       if constexpr (!CHOOSE) {
-        O* o = (O*)a.out + row * a.out_stride + v;
-        if (left >= 4) Elt<O>::store4(o, x[q]);
+        O* o = (O*)((char*)a.out + row * a.out_stride * (long long)sizeof(O) + v * (unsigned)sizeof(O));
+        const f32x4 to = {x[q][0], x[q][1], x[q][2], x[q][3]};
+        if (left >= 4) Elt<O>::store4(o, to);
         else {
-          if (left > 0) o[0] = Elt<O>::put(x[q][0]);
-          if (left > 1) o[1] = Elt<O>::put(x[q][1]);
-          if (left > 2) o[2] = Elt<O>::put(x[q][2]);
+          if (left > 0) o[0] = Elt<O>::put(to[0]);
+          if (left > 1) o[1] = Elt<O>::put(to[1]);
+          if (left > 2) o[2] = Elt<O>::put(to[2]);
         }
       } else {
+        float key[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float y = sampled ? x[q][i] * inv : x[q][i];
-          const float key = sampled ? y + g[q][i] : y;
-          const bool better = key > ch.key;                 // the first of equal keys stays; against a NaN nothing is better
-          ch.key = better ? key : ch.key;
-          ch.y = better ? y : ch.y;
-          ch.v = better ? v + i : ch.v;
-          bm = fmaxf(bm, y);
-          x[q][i] = y;
+          x[q][i] = x[q][i] * inv;                          // a greedy row: times 1, plus 0
+          key[i] = x[q][i] + g[q][i];
+        }
+        top[q] = max_of<4>(x[q], NINF);
+        // A later quad of the wave has the greater indices, so only what is ahead of every lane's best counts; that soon becomes rare
+        if (__builtin_amdgcn_ballot_w64(max_of<4>(key, NINF) > ahead) != 0) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool better = key[i] > ch.key;            // the first of equal keys stays; against a NaN nothing is better
+            ch.key = better ? key[i] : ch.key;
+            ch.y = better ? x[q][i] : ch.y;
+            ch.v = better ? v + i : ch.v;
+          }
+          ahead = wave_reduce<MaxOp>(ch.key);
         }
       }
       __builtin_amdgcn_sched_barrier(0);                    // one quad at a time: 64 registers let two workgroups of 1024 share a CU
     }
     if constexpr (CHOOSE) {
-      if (bm > ch.m) {
+      // The sum's shift need not be the maximum: it follows once that is 30 ahead, where the exponentials (below 2^44) are far from overflowing
+      const float bm = fmaxf(top[0], top[1]);
+      if (bm > ch.m + 30.0f) {
         if (ch.m != NINF) ch.s *= Shift(bm, LOG2E).from(Shift(ch.m, LOG2E));
         ch.m = bm;
       }
-      const Shift sh(ch.m == NINF ? 0.0f : ch.m, LOG2E);
+      Shift sh(ch.m == NINF ? 0.0f : ch.m, LOG2E);
+      sh.fast = __builtin_amdgcn_ballot_w64(!sh.fast) == 0;
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         float e[4] = {x[q][0], x[q][1], x[q][2], x[q][3]};
@@ -348,7 +365,10 @@ __global__ void __launch_bounds__(G == 64 ? 256 : G, 8) frl_logits_kernel(const 
         }
       }
     }
-  }
+  };
+  for (int c = c0; c < min(c1, whole); ++c) chunk(c, std::true_type());
+  if (c1 > whole) chunk(whole, std::false_type());
+
   if constexpr (CHOOSE) {
     const float m = group_reduce<MaxOp, G>(ch.m, red_m);
     if (ch.m != NINF) ch.s *= Shift(m, LOG2E).from(Shift(ch.m, LOG2E));
@@ -397,14 +417,17 @@ __global__ void __launch_bounds__(256) frl_logits_join_kernel(const LogitsArgs a
 
 struct LogitsPlan { int G, chunks, per, parts; };
 
-// Threads per chunk: a wave for short rows; a workgroup of 1024 where that gives every CU two of them (the history is then searched for the fewest
-// chunks); else 256, which spreads a few rows over more CUs.  A group takes so many chunks of a row that about two rounds of resident groups remain.
+// Threads per chunk: a wave for short rows; a workgroup of 1024 where lists have to be searched for every chunk and the batch gives every CU two such
+// workgroups; else 256.  A group takes so many chunks of a row that about one round (1024 threads) or two (256) of resident groups remain.  Measured,
+// bf16 choice of 256 x 131072: with a history of 4096, 68 us by 1024 threads in 512 groups, 75 in 1024 groups, 90 by 256 threads in 4096;
+// without lists 39 us by 1024 threads, 37.5 by 256.
 static LogitsPlan logits_plan(const FrlLogitsDesc* d) {
   LogitsPlan p;
   const long long wide = d->rows * (((long long)d->vocab + 8191) / 8192);
-  p.G = d->vocab <= 512 && d->n_sparse <= 512 ? 64 : (d->vocab > 4096 && wide >= 512) ? 1024 : 256;
+  const bool lists = d->history_len > 0 || d->n_sparse > 0;
+  p.G = d->vocab <= 512 && d->n_sparse <= 512 ? 64 : (lists && d->vocab > 4096 && wide >= 512) ? 1024 : 256;
   p.chunks = (int)((d->vocab + 8LL * p.G - 1) / (8 * p.G));
-  const long long rounds = d->rows * p.chunks / (p.G == 1024 ? 1024 : 4096);
+  const long long rounds = d->rows * p.chunks / (p.G == 1024 ? 512 : 4096);
   p.per = rounds < 1 ? 1 : rounds > p.chunks ? p.chunks : (int)rounds;
   p.parts = (p.chunks + p.per - 1) / p.per;
   p.per = (p.chunks + p.parts - 1) / p.parts;
@@ -461,17 +484,18 @@ static int logits_fill(const FrlLogitsDesc* d, const FrlLogitsBufs* b, LogitsArg
                  b->bias, b->bias_tokens, b->bias_values, b->allowed, b->temperature, b->gumbel, b->token, b->logprob,
                  nullptr, nullptr, nullptr, nullptr,
                  d->logits_stride, d->out_stride, d->gumbel_stride, d->history_stride, d->bias_stride, d->sparse_stride, d->mask_stride,
-                 d->repetition, d->frequency, d->presence, d->temperature, d->vocab, d->ids64, d->history_len, d->n_sparse, d->mask, 0, 0, 0, 0};
+                 d->repetition, d->frequency, d->presence, d->temperature, d->vocab, d->ids64, d->history_len, d->n_sparse, d->mask, 0, 0, 0, 0, 0};
   const LogitsPlan p = logits_plan(d);
   G = p.G;
   a.chunks = p.chunks; a.per = p.per; a.parts = p.parts;
   a.items = (long long)d->rows * p.parts;
+  a.eager = a.items * p.G < 2048LL * 1024 || p.G == 64;      // less than two waves for every slot of the chip, or rows shorter than what skipping saves
   return FRL_OK;
 }
 
 static size_t logits_workspace(const FrlLogitsDesc* d) {
   const int parts = logits_plan(d).parts;
-  return ((parts > 1 ? (size_t)d->rows * parts * 20 : 0) + 511) / 256 * 256;
+  return parts > 1 ? ((size_t)d->rows * parts * 20 + 511) / 256 * 256 : 256;
 }
 
 }  // namespace frl

@@ -63,6 +63,8 @@ class Constraints:
 
 
 _NO_RULES = Constraints()
+# torch.cuda.current_stream(index).cuda_stream, without the Stream object where torch has the shorter way
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 # A decoding step's call is as short as its host side.  The C structs are therefore filled with one pack each (their ctypes layout,
 # checked here once) and every operand takes one cheap test on the way to its pointer; only an operand that fails it is looked at closely.
@@ -219,7 +221,7 @@ def _marshal(z: torch.Tensor, R: int, V: int, c: Constraints, z_stride: Optional
 
 def _call(fn, index: int, *args) -> None:
     """The entry point on the device's current stream, with the device as the current one while it is called."""
-    stream = torch.cuda.current_stream(index).cuda_stream
+    stream = _current_stream(index)
     if torch.cuda.current_device() == index:
         rc = fn(*args, stream)
     else:
@@ -240,7 +242,7 @@ def constrain(logits: torch.Tensor, rules: Optional[Constraints] = None, *, out:
     index = logits.get_device()
     if out is None:
         dtype = logits.dtype if out_dtype is None else out_dtype
-        out = torch.empty(logits.shape, dtype=dtype, device=logits.device)
+        out = torch.empty_like(logits, dtype=dtype, memory_format=torch.contiguous_format)
         o_stride = V
     else:
         dtype = out.dtype
@@ -293,8 +295,8 @@ def choose(logits: torch.Tensor, rules: Optional[Constraints] = None, *, tempera
     lib = _lib.load()
     # a tensor of this call's own: calls on two streams, and graphs captured from them, share no scratch
     need = lib.frl_logits_workspace_bytes(C.byref(d))
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _call(lib.frl_logits_choose, index, C.byref(d), C.byref(b), ws.data_ptr() if need else None, need)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 256 else None
+    _call(lib.frl_logits_choose, index, C.byref(d), C.byref(b), None if ws is None else ws.data_ptr(), need)
     return token, logprob
 
 
@@ -327,7 +329,7 @@ def distill_forward(logits, ids, teacher, kind, temperature, weights, reduction,
         raise RuntimeError("flowrl_hip runs on the GPU only; there is no CPU fallback")
     dev, lead = logits.device, logits.shape[:-1]
     loss = torch.empty(lead if reduction == "none" else (), dtype=torch.float32, device=dev)
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if want_grad else None
+    grad = torch.empty_like(logits, memory_format=torch.contiguous_format) if want_grad else None
     stats = torch.empty((math.prod(lead) + 1, _lib.FRL_DISTILL_STATS), dtype=torch.float32, device=dev) if want_stats else None
     d, b, keep = _distill_marshal(logits, ids, teacher, kind, temperature, weights, reduction, loss.data_ptr(), stats.data_ptr() if want_stats else 0, 0,
                                   grad.data_ptr() if want_grad else 0)
@@ -342,7 +344,7 @@ def distill_forward(logits, ids, teacher, kind, temperature, weights, reduction,
 
 def distill_backward(logits, ids, teacher, kind, temperature, weights, reduction, stats, g_loss):
     """d loss / d logits times ``g_loss`` from the forward's row statistics: frl_distill_bwd."""
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    grad = torch.empty_like(logits, memory_format=torch.contiguous_format)
     index = logits.get_device()
     g = _row_values(g_loss, math.prod(logits.shape[:-1]) if reduction == "none" else 1, index, torch.float32, "g_loss")
     d, b, keep = _distill_marshal(logits, ids, teacher, kind, temperature, weights, reduction, 0, stats.data_ptr(), g.data_ptr(), grad.data_ptr())

@@ -524,7 +524,8 @@ int frl_logits_constrain(const FrlLogitsDesc* desc, const FrlLogitsBufs* bufs, v
 /* One entry per row of the constrained logits, without writing them.  With T = temperature > 0 and noise: y = x * (1 /
  * (1e-6 + T)) and token = argmax(y + gumbel), the categorical draw of frl_critic_select; else y = x and token = argmax(y).
  * The first of equal maxima; a NaN counts as the largest value (argmax's rule in jax and torch).  logprob = y[token] -
- * log sum exp y.  A row that its rules leave nothing (every y is -inf) answers token -1, logprob -inf. */
+ * log sum exp y.  A row that its rules leave nothing (every y is -inf) answers token -1, logprob -inf.
+ * frl_logits_workspace_bytes: 0 for a bad descriptor; 256 where a call needs no scratch and takes workspace = NULL. */
 size_t frl_logits_workspace_bytes(const FrlLogitsDesc* desc);
 int frl_logits_choose(const FrlLogitsDesc* desc, const FrlLogitsBufs* bufs, void* workspace, size_t workspace_bytes, void* hip_stream);
 
