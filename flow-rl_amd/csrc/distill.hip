@@ -21,7 +21,6 @@ struct DistillArgs {
   float* rowloss;             // (rows,) weight * L
   float* stats;               // (rows + 1, 4) or NULL: m, 1 / s, factor of the named entries, factor of the others; last row: 1 / denominator
   const float* inv_denom;     // device 1 / sum of weights, or NULL: `denom_scale`
-  int sum_weights;            // row kernel: every group sums the weights itself
   const float* g_loss;        // backward: cotangent, `g_stride` apart per row (0: one scalar); NULL: 1
   void* grad;
   float* part;                // split rows: (rows, segs, 3) m, s, r
@@ -296,14 +295,14 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, 4) frl_distill_row_kernel(c
   constexpr int GPB = G <= 64 ? 256 / G : 1, N = Vec16<T>::N;
   constexpr int WAVES = G < 64 ? 1 : G / 64;
   __shared__ float red0[WAVES], red1[WAVES];
-  __shared__ double row_p[GPB], row_x[GPB], red2[WAVES];
+  __shared__ double row_p[GPB], row_x[GPB];
   const int tid = threadIdx.x % G, grp = G < 64 ? threadIdx.x / G : G == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
   const int nwords = REST ? (a.vocab + 31) / 32 : 0;
   unsigned* words = lds + (size_t)grp * (nwords + 3 * a.top);
   int* sid = (int*)(words + nwords);
   float* sp = (float*)(sid + a.top);
   float* sz = sp + a.top;
-  float inv = a.inv_denom != nullptr ? *a.inv_denom : a.denom_scale;
+  const float inv = a.inv_denom != nullptr ? *a.inv_denom : a.denom_scale;
   const int nvec = a.vocab / N, tail = a.vocab - nvec * N, nv = (nvec + G - 1) / G;
   const long long row = block_index() * GPB + grp;
   if (row >= a.rows) return;
@@ -332,11 +331,6 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, 4) frl_distill_row_kernel(c
     double sum_p, cross;
     teacher_part<T, G < 64 ? G : 64, REST>(a, row, z, tid, sid, sp, sz, sum_p, cross);
     if (tid == 0) { row_p[grp] = sum_p; row_x[grp] = cross; }
-  }
-  if (GRAD && a.sum_weights) {                              // an eighth of the row's bytes at most, out of the cache, while the row is on its way
-    double sw = 0.0;
-    for (long long i = t0; i < a.rows; i += G) sw += (double)a.weights[i];
-    inv = inverse(group_reduce<SumOp, G>(sw, red2));
   }
   Running<REST> run;
   if (nvec > NV * G) run.template stream<T, G>(z, NV * G, nvec, a.scale2, words, t0);
@@ -542,7 +536,7 @@ __device__ __forceinline__ double sum_of_rows(const float* __restrict__ x, long 
   return wave_reduce<SumOp>(threadIdx.x < 16 ? red[threadIdx.x] : 0.0);
 }
 
-// 1 / sum of the weights, 0 where the sum is 0: ahead of a gradient that is too short to sum them itself
+// 1 / sum of the weights, 0 where the sum is 0: ahead of a gradient
 __global__ void __launch_bounds__(1024) frl_distill_denom_kernel(const float* __restrict__ w, long long rows, float* __restrict__ inv) {
   const double s = sum_of_rows(w, rows);
   if (threadIdx.x == 0) *inv = inverse(s);
@@ -741,19 +735,12 @@ int frl_distill_fwd(const FrlDistillDesc* desc, const FrlDistillBufs* bufs, void
   hipError_t e = hipSuccess;
   const bool reduce = desc->reduction != FRL_REDUCE_NONE, weighted = desc->reduction == FRL_REDUCE_MEAN && bufs->weights != nullptr && desc->rows > 0;
   float* inv = weighted ? (bufs->row_stats != nullptr ? bufs->row_stats + 4 * desc->rows : ws + w.inv) : nullptr;
-  // A gradient needs the weights' sum before it starts.  Rows of eight times the weights' bytes sum them
-  // in every group (8192 x 131072 bf16: 940 against 948 + 5 us); at less a kernel of its own does (4096 x 32000: 115 + 5 against 132 us).
-  const size_t elt = desc->dtype == FRL_ELT_F32 ? 4 : 2;
   const bool finish = split && reduce && desc->rows <= 16 && desc->top * desc->rows * 12 <= 48 * 1024;     // the join is one workgroup and finishes the loss
-  bool have_inv = false;
-  if (weighted && grad && !split) {
-    a.sum_weights = (size_t)desc->rows * 4 * 8 <= (size_t)desc->vocab * elt;
-    if (!a.sum_weights) {
-      hipLaunchKernelGGL(frl_distill_denom_kernel, dim3(1), dim3(1024), 0, st, bufs->weights, (long long)desc->rows, inv);
-      e = hipGetLastError();
-      note_kernel("frl_distill_denom_kernel");
-      have_inv = true;
-    }
+  const bool have_inv = weighted && grad && !split;          // a gradient needs the weights' sum before it starts; else the last kernel adds them up
+  if (have_inv) {
+    hipLaunchKernelGGL(frl_distill_denom_kernel, dim3(1), dim3(1024), 0, st, bufs->weights, (long long)desc->rows, inv);
+    e = hipGetLastError();
+    note_kernel("frl_distill_denom_kernel");
   }
   a.inv_denom = have_inv ? inv : nullptr;
   if (e == hipSuccess && desc->rows > 0) {

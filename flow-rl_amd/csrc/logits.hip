@@ -297,17 +297,21 @@ __global__ void __launch_bounds__(G == 64 ? 256 : G, 8) frl_logits_kernel(const 
       for (int i = 0; i < 4; ++i) {
         float t = in[i];
         const unsigned word = (unsigned)w4[i];
-        if (HIST && word != 0u) {                           // few tokens are listed: often no lane of a wave has one, and the wave skips this
-          const unsigned count = SPARSE ? word & COUNT_MASK : word & ~SEEN_IN_PROMPT;
-          const unsigned seen = SPARSE ? word & (SEEN_IN_PROMPT | COUNT_MASK) : word;
-          const float pushed = t > 0.0f ? divide(t, rep, rrep) : t * rep;
-          t = seen != 0u ? pushed : t;
-          t = t - (freq * (float)count + (count != 0u ? pres : 0.0f));
-        }
-        if (a.bias != nullptr) t = t + b[i];
-        if constexpr (SPARSE) {
-          const unsigned slot = word >> SLOT_SHIFT & SLOT_MASK;
-          if (slot != 0u) t = t + val[slot - 1u];
+        if (WORDS && word != 0u) {                          // few tokens are listed: often no lane of a wave has one, and the wave skips this
+          if constexpr (HIST) {
+            const unsigned count = SPARSE ? word & COUNT_MASK : word & ~SEEN_IN_PROMPT;
+            const unsigned seen = SPARSE ? word & (SEEN_IN_PROMPT | COUNT_MASK) : word;
+            const float pushed = t > 0.0f ? divide(t, rep, rrep) : t * rep;
+            t = seen != 0u ? pushed : t;
+            t = t - (freq * (float)count + (count != 0u ? pres : 0.0f));
+          }
+          if (a.bias != nullptr) t = t + b[i];
+          if constexpr (SPARSE) {
+            const unsigned slot = word >> SLOT_SHIFT & SLOT_MASK;
+            if (slot != 0u) t = t + val[slot - 1u];
+          }
+        } else if (a.bias != nullptr) {
+          t = t + b[i];
         }
         const unsigned keep = (unsigned)((int)(now[q] << (31 - i)) >> 31);
         x[q][i] = __uint_as_float((__float_as_uint(t) & keep) | (0xff800000u & ~keep));
