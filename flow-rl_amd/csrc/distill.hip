@@ -599,7 +599,7 @@ static int distill_validate(const FrlDistillDesc* d) {
   if (d->kind < FRL_DISTILL_TOP || d->kind > FRL_DISTILL_REST) { set_error("distill: kind %d invalid", d->kind); return FRL_EINVAL; }
   if (d->reduction < FRL_REDUCE_NONE || d->reduction > FRL_REDUCE_MEAN) { set_error("distill: reduction %d invalid", d->reduction); return FRL_EINVAL; }
   if (d->rows < 0 || d->vocab < 1 || d->top < 1) { set_error("distill: rows %lld / vocab %d / top %d invalid", (long long)d->rows, d->vocab, d->top); return FRL_EINVAL; }
-  if (!(d->temperature > 0.0f)) { set_error("distill: temperature %g must be > 0", d->temperature); return FRL_EINVAL; }
+  if (!(d->temperature >= 1e-30f && d->temperature <= 1e30f)) { set_error("distill: temperature %g outside [1e-30, 1e30]", d->temperature); return FRL_EINVAL; }
   if (d->top > FRL_DISTILL_MAX_TOP) { set_error("distill: top %d > %d", d->top, FRL_DISTILL_MAX_TOP); return FRL_EUNSUPPORTED; }
   if (d->vocab > (1 << 30)) { set_error("distill: vocab %d > 2^30", d->vocab); return FRL_EUNSUPPORTED; }
   if (d->rows > (1LL << 30)) { set_error("distill: %lld rows > 2^30", (long long)d->rows); return FRL_EUNSUPPORTED; }

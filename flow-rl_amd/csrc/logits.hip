@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(G == 64 ? 256 : G, 8) frl_logits_kernel(const 
   const T* z = (const T*)a.logits + row * a.logits_stride;
   const float temp = !CHOOSE ? 0.0f : a.temperature != nullptr ? a.temperature[row] : a.temp;
   const bool sampled = CHOOSE && a.gumbel != nullptr && temp > 0.0f;
-  const float inv = sampled ? 1.0f / (1e-6f + temp) : 1.0f;
+  const float inv = sampled ? fmaxf(1.0f / (1e-6f + temp), 1.17549435e-38f) : 1.0f;      // never 0: an infinite temperature leaves -inf what it is
   const float* noise = sampled ? a.gumbel + row * a.gumbel_stride : nullptr;
 
   const void* mask = a.mask == FRL_MASK_WORDS ? (const void*)((const unsigned*)a.allowed + row * a.mask_stride) : (const void*)((const unsigned char*)a.allowed + row * a.mask_stride);

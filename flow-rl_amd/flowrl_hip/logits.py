@@ -63,7 +63,9 @@ class Constraints:
 
 
 _NO_RULES = Constraints()
-# torch.cuda.current_stream(index).cuda_stream, without the Stream object where torch has the shorter way
+# torch.cuda.current_stream(index).cuda_stream without the Stream object, and torch.cuda.current_device() without its initialisation check (the logits
+# are on the device already), where torch has the shorter ways
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 # A decoding step's call is as short as its host side.  The C structs are therefore filled with one pack each (their ctypes layout,
@@ -126,81 +128,85 @@ def _rows_of(t: torch.Tensor, R: int, n: int, index: int, what: str, shared: boo
     return t, t.stride(0)
 
 
+_IDS = {torch.int32: 0, torch.int64: 1}
+
+
 def _ids(t: torch.Tensor, what: str) -> int:
     """1 for int64 tokens, 0 for int32"""
-    if t.dtype is torch.int32:
-        return 0
-    if t.dtype is torch.int64:
-        return 1
-    raise TypeError(f"{what}: int32 or int64 tokens required (got {t.dtype})")
+    wide = _IDS.get(t.dtype)
+    if wide is None:
+        raise TypeError(f"{what}: int32 or int64 tokens required (got {t.dtype})")
+    return wide
 
 
 def _no_grad(what: str, *ts) -> None:
     for t in ts:
-        if t is not None and t.requires_grad:
+        if isinstance(t, torch.Tensor) and t.requires_grad:
             raise NotImplementedError(f"flowrl_hip.logits: {what} is not differentiated here; detach it")
+
+
+def _differentiable(c: Constraints):
+    return c.bias, c.bias_values, c.repetition, c.frequency, c.presence
 
 
 def _marshal(z: torch.Tensor, R: int, V: int, c: Constraints, z_stride: Optional[int] = None, out_elt: int = 0, out_stride: int = 0, out: int = 0,
              temperature: float = 0.0, temperature_ptr: int = 0, gumbel_stride: int = 0, gumbel: int = 0, token: int = 0, logprob: int = 0):
     """FrlLogitsDesc / FrlLogitsBufs of one call, and the copies that they point into."""
-    index, keep = z.get_device(), []
+    index, keep = z.get_device(), ()
     ids64 = L = K = mask = h_stride = b_stride = s_stride = m_stride = 0
-    h_ptr = b_ptr = t_ptr = v_ptr = a_ptr = 0
-    rows = [0, 0, 0, 0, 0]                  # lengths, prompt_lengths, repetition, frequency, presence
+    h_ptr = len_ptr = prompt_ptr = rep_ptr = freq_ptr = pres_ptr = b_ptr = t_ptr = v_ptr = a_ptr = 0
     rep, freq, pres = 1.0, 0.0, 0.0
     history, tokens, values = c.history, c.bias_tokens, c.bias_values
-    if history is not None and tokens is not None and history.dtype is not tokens.dtype:
-        _ids(history, "history"), _ids(tokens, "bias_tokens")
-        history, tokens = history.long(), tokens.long()
+    lengths, prompt = c.lengths, c.prompt_lengths
     if history is not None:
+        if tokens is not None and history.dtype is not tokens.dtype:
+            _ids(history, "history"), _ids(tokens, "bias_tokens")
+            history, tokens = history.long(), tokens.long()
         ids64 = _ids(history, "history")
         L = history.shape[-1] if history.dim() else 0
         history, h_stride = _rows_of(history, R, L, index, "history", False)
-        keep.append(history)
         h_ptr = history.data_ptr()
-        if c.lengths is not None:
-            t = _row_values(c.lengths, R, index, torch.int32, "lengths")
-            keep.append(t)
-            rows[0] = t.data_ptr()
-        if c.prompt_lengths is not None:
-            t = _row_values(c.prompt_lengths, R, index, torch.int32, "prompt_lengths")
-            keep.append(t)
-            rows[1] = t.data_ptr()
+        if lengths is not None:
+            lengths = _row_values(lengths, R, index, torch.int32, "lengths")
+            len_ptr = lengths.data_ptr()
+        if prompt is not None:
+            prompt = _row_values(prompt, R, index, torch.int32, "prompt_lengths")
+            prompt_ptr = prompt.data_ptr()
         rep, freq, pres = c.repetition, c.frequency, c.presence
+        keep = [history, lengths, prompt]
         if isinstance(rep, torch.Tensor):
             t = _row_values(rep, R, index, torch.float32, "repetition")
+            rep_ptr, rep = t.data_ptr(), 1.0
             keep.append(t)
-            rows[2], rep = t.data_ptr(), 1.0
         if isinstance(freq, torch.Tensor):
             t = _row_values(freq, R, index, torch.float32, "frequency")
+            freq_ptr, freq = t.data_ptr(), 0.0
             keep.append(t)
-            rows[3], freq = t.data_ptr(), 0.0
         if isinstance(pres, torch.Tensor):
             t = _row_values(pres, R, index, torch.float32, "presence")
+            pres_ptr, pres = t.data_ptr(), 0.0
             keep.append(t)
-            rows[4], pres = t.data_ptr(), 0.0
-    elif c.lengths is not None or c.prompt_lengths is not None:
+    elif lengths is not None or prompt is not None:
         raise ValueError("lengths / prompt_lengths without a history")
-    if c.bias is not None:
-        if c.bias.dtype is not torch.float32:
-            raise TypeError(f"bias: float32 required (got {c.bias.dtype})")
-        t, b_stride = _rows_of(c.bias, R, V, index, "bias", True)
-        keep.append(t)
-        b_ptr = t.data_ptr()
-    if (tokens is None) != (values is None):
-        raise ValueError("bias_tokens and bias_values come together")
+    bias = c.bias
+    if bias is not None:
+        if bias.dtype is not torch.float32:
+            raise TypeError(f"bias: float32 required (got {bias.dtype})")
+        bias, b_stride = _rows_of(bias, R, V, index, "bias", True)
+        b_ptr = bias.data_ptr()
     if tokens is not None:
-        if values.dtype is not torch.float32 or values.shape != tokens.shape:
-            raise TypeError(f"bias_values: float32 of bias_tokens' shape {tuple(tokens.shape)} required (got {tuple(values.shape)} of {values.dtype})")
+        if values is None or values.dtype is not torch.float32 or values.shape != tokens.shape:
+            got = "none" if values is None else f"{tuple(values.shape)} of {values.dtype}"
+            raise (ValueError if values is None else TypeError)(f"bias_values: float32 of bias_tokens' shape {tuple(tokens.shape)} required (got {got})")
         ids64 = _ids(tokens, "bias_tokens")
         K = tokens.shape[-1] if tokens.dim() else 0
         tokens, s_stride = _rows_of(tokens, R, K, index, "bias_tokens", True)
         values, stride = _rows_of(values, R, K, index, "bias_values", True)
         if stride != s_stride:
             tokens, values, s_stride = tokens.contiguous(), values.contiguous(), K
-        keep += (tokens, values)
         t_ptr, v_ptr = tokens.data_ptr(), values.data_ptr()
+    elif values is not None:
+        raise ValueError("bias_values without bias_tokens")
     allowed = c.allowed
     if allowed is not None:
         if allowed.dtype is torch.bool:
@@ -210,19 +216,18 @@ def _marshal(z: torch.Tensor, R: int, V: int, c: Constraints, z_stride: Optional
         else:
             raise TypeError(f"allowed: bool entries or int32 words of 32 entries required (got {allowed.dtype})")
         allowed, m_stride = _rows_of(allowed, R, n, index, "allowed", True)
-        keep.append(allowed)
         a_ptr = allowed.data_ptr()
     d, b = _lib.FrlLogitsDesc(), _lib.FrlLogitsBufs()
     _DESC.pack_into(d, 0, _lib.FRL_ABI_VERSION, _ELT[z.dtype], out_elt, V, R, ids64, L, K, mask, V if z_stride is None else z_stride, out_stride, gumbel_stride,
                     h_stride, b_stride, s_stride, m_stride, rep, freq, pres, temperature)
-    _BUFS.pack_into(b, 0, z.data_ptr(), out, h_ptr, *rows, b_ptr, t_ptr, v_ptr, a_ptr, temperature_ptr, gumbel, token, logprob)
-    return d, b, keep
+    _BUFS.pack_into(b, 0, z.data_ptr(), out, h_ptr, len_ptr, prompt_ptr, rep_ptr, freq_ptr, pres_ptr, b_ptr, t_ptr, v_ptr, a_ptr, temperature_ptr, gumbel, token, logprob)
+    return d, b, (keep, bias, tokens, values, allowed)
 
 
 def _call(fn, index: int, *args) -> None:
     """The entry point on the device's current stream, with the device as the current one while it is called."""
     stream = _current_stream(index)
-    if torch.cuda.current_device() == index:
+    if _current_device() == index:
         rc = fn(*args, stream)
     else:
         with torch.cuda.device(index):
@@ -237,7 +242,7 @@ def constrain(logits: torch.Tensor, rules: Optional[Constraints] = None, *, out:
     tensor of the logits' shape with contiguous rows; it may be ``logits`` itself."""
     rules = _NO_RULES if rules is None else rules
     if torch.is_grad_enabled():
-        _no_grad("logits / bias", logits, rules.bias, rules.bias_values)
+        _no_grad("logits / a rule", logits, *_differentiable(rules))
     z, R, V, stride = _check_logits(logits, "logits")
     index = logits.get_device()
     if out is None:
@@ -266,16 +271,16 @@ def constrain(logits: torch.Tensor, rules: Optional[Constraints] = None, *, out:
 def choose(logits: torch.Tensor, rules: Optional[Constraints] = None, *, temperature: PerRow = 0.0,
            gumbel: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """One entry per row of the constrained logits and its log-probability: (token int32, logprob float32) of the logits'
-    leading shape.  Rows with ``temperature`` (a number, or float32 (rows,)) <= 0 take the argmax; the others draw
+    leading shape.  Rows whose ``temperature`` (a number, or float32 (rows,)) is not > 0 take the argmax; the others draw
     argmax(y + gumbel) with y = logits / (1e-6 + temperature) and ``gumbel`` (rows, vocab) float32 Gumbel(0, 1) noise, finite
     (:func:`flowrl_hip.random.gumbel`); without noise every row is greedy, and a number > 0 for the temperature is refused.  The
     first of equal maxima; NaN counts as the largest.  logprob is log softmax of y (of the constrained logits for a greedy row).  A row
     that the rules leave nothing answers token -1 with logprob -inf."""
     rules = _NO_RULES if rules is None else rules
     if torch.is_grad_enabled():
-        _no_grad("logits / bias", logits, rules.bias, rules.bias_values)
+        _no_grad("logits / a rule / the temperature", logits, temperature, *_differentiable(rules))
     z, R, V, stride = _check_logits(logits, "logits")
-    index, dev = logits.get_device(), logits.device
+    index = logits.get_device()
     t = g = None
     t_ptr = g_ptr = g_stride = 0
     if isinstance(temperature, torch.Tensor):
@@ -289,13 +294,13 @@ def choose(logits: torch.Tensor, rules: Optional[Constraints] = None, *, tempera
             g, g_stride = g.contiguous(), V
         g_ptr = g.data_ptr()
     lead = logits.shape[:-1]
-    token = torch.empty(lead, dtype=torch.int32, device=dev)
-    logprob = torch.empty(lead, dtype=torch.float32, device=dev)
+    token = logits.new_empty(lead, dtype=torch.int32)
+    logprob = logits.new_empty(lead, dtype=torch.float32)
     d, b, keep = _marshal(z, R, V, rules, stride, 0, 0, 0, temperature, t_ptr, g_stride, g_ptr, token.data_ptr(), logprob.data_ptr())
     lib = _lib.load()
     # a tensor of this call's own: calls on two streams, and graphs captured from them, share no scratch
     need = lib.frl_logits_workspace_bytes(C.byref(d))
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 256 else None
+    ws = logits.new_empty(need, dtype=torch.uint8) if need > 256 else None
     _call(lib.frl_logits_choose, index, C.byref(d), C.byref(b), None if ws is None else ws.data_ptr(), need)
     return token, logprob
 
@@ -327,17 +332,17 @@ def distill_forward(logits, ids, teacher, kind, temperature, weights, reduction,
         raise ValueError(f"reduction {reduction!r}: 'mean', 'sum' or 'none'")
     if not logits.is_cuda:
         raise RuntimeError("flowrl_hip runs on the GPU only; there is no CPU fallback")
-    dev, lead = logits.device, logits.shape[:-1]
-    loss = torch.empty(lead if reduction == "none" else (), dtype=torch.float32, device=dev)
+    lead = logits.shape[:-1]
+    loss = logits.new_empty(lead if reduction == "none" else (), dtype=torch.float32)
     grad = torch.empty_like(logits, memory_format=torch.contiguous_format) if want_grad else None
-    stats = torch.empty((math.prod(lead) + 1, _lib.FRL_DISTILL_STATS), dtype=torch.float32, device=dev) if want_stats else None
+    stats = logits.new_empty((math.prod(lead) + 1, _lib.FRL_DISTILL_STATS), dtype=torch.float32) if want_stats else None
     d, b, keep = _distill_marshal(logits, ids, teacher, kind, temperature, weights, reduction, loss.data_ptr(), stats.data_ptr() if want_stats else 0, 0,
                                   grad.data_ptr() if want_grad else 0)
     if reduction == "none" and loss.numel() == 0:
         return loss, grad, stats
     lib = _lib.load()
     need = lib.frl_distill_workspace_bytes(C.byref(d))
-    ws = torch.empty(need or 256, dtype=torch.uint8, device=dev)       # need == 0: the entry point says why
+    ws = logits.new_empty(need or 256, dtype=torch.uint8)              # need == 0: the entry point says why
     _call(lib.frl_distill_fwd, logits.get_device(), C.byref(d), C.byref(b), ws.data_ptr(), need)
     return loss, grad, stats
 

@@ -356,7 +356,7 @@ double frl_hoisted_flops(const FrlDesc* desc);
 /* Thread-local message of the last failing call on this thread ("" if none). */
 const char* frl_last_error(void);
 
-/* Diagnostics (no reference counterpart): the compute kernels the LAST sampler / VJP / evaluation / critic entry point called
+/* Diagnostics (no reference counterpart): the compute kernels the LAST sampler / VJP / evaluation / critic / logits / distill entry point called
  * on this thread actually enqueued, as "name<instantiation> [grid] + ..." (thread-local; "" before any call).  Written by
  * the launchers themselves, so a benchmark that reports which build ran cannot drift from the dispatch rules. */
 const char* frl_last_kernels(void);
@@ -522,7 +522,7 @@ typedef struct FrlLogitsBufs {
 int frl_logits_constrain(const FrlLogitsDesc* desc, const FrlLogitsBufs* bufs, void* hip_stream);
 
 /* One entry per row of the constrained logits, without writing them.  With T = temperature > 0 and noise: y = x * (1 /
- * (1e-6 + T)) and token = argmax(y + gumbel), the categorical draw of frl_critic_select; else y = x and token = argmax(y).
+ * (1e-6 + T)) (the factor at least FLT_MIN) and token = argmax(y + gumbel), the categorical draw of frl_critic_select; else y = x and token = argmax(y).
  * The first of equal maxima; a NaN counts as the largest value (argmax's rule in jax and torch).  logprob = y[token] -
  * log sum exp y.  A row that its rules leave nothing (every y is -inf) answers token -1, logprob -inf.
  * frl_logits_workspace_bytes: 0 for a bad descriptor; 256 where a call needs no scratch and takes workspace = NULL. */
@@ -558,7 +558,7 @@ typedef struct FrlDistillDesc {
   int32_t vocab, top;
   int64_t rows;
   int64_t logits_stride, grad_stride, ids_stride, teacher_stride;
-  float temperature; /* > 0 */
+  float temperature; /* in [1e-30, 1e30] */
 } FrlDistillDesc;
 
 typedef struct FrlDistillBufs {

@@ -79,6 +79,10 @@ CASES = [
     (300, 8195, dict(hist=130, prompt=True, sparse=33), "words"),          # workgroups of 1024 threads
     (520, 5003, dict(hist=64, dense="shared"), "bool"),
     (600, 4097, dict(), None),
+    (600, 5003, dict(hist=16, sparse=2048), None),                          # the longest lists beside 1024 threads
+    (2, 40, dict(hist=9, sparse=2048), "bool"),                             # lists far longer than the row
+    (3, 70001, dict(hist=9000, prompt=True, sparse=600, wide=True), "bool"),   # a history that no group keeps in registers
+    (560, 9001, dict(hist=5000, prompt=True), None),
 ]
 IDS = [f"{R}x{V}-{'-'.join(k for k in kw)}-{mask}" for R, V, kw, mask in CASES]
 
@@ -145,6 +149,28 @@ def test_ties_take_the_first(V):
     assert token.tolist() == [0, V // 2, 0, V - 1]
     # every exponential is exact and so are their sums up to 2^24: only the logarithm and one subtraction round
     assert abs(float(logprob[0]) + np.log(V)) <= 2.0 ** -22 * (1 + np.log(V))
+
+
+@pytest.mark.parametrize("R,V", [(1, 5000), (40, 33000), (700, 9000)])
+def test_extreme_temperatures(R, V):
+    """From the argmax of the noise (infinite temperature, what is not allowed stays out) to that of the logits (tiny)."""
+    import torch
+    import flowrl_hip as fh
+    rng = np.random.default_rng(V)
+    z = _logits(rng, R, V, torch.float32).cuda()
+    g = torch.from_numpy(rng.gumbel(size=(R, V)).astype(np.float32)).cuda()
+    allowed = torch.rand((R, V), device="cuda") < 0.5
+    rules = fh.logits.Constraints(allowed=allowed)
+    x = torch.where(allowed, z, -torch.inf)
+    token, logprob = fh.logits.choose(z, rules, temperature=float("inf"), gumbel=g)
+    assert torch.equal(token.long(), torch.where(x == -torch.inf, -torch.inf, g).argmax(1))
+    n = (x > -torch.inf).sum(1).double().cpu().numpy()
+    assert (np.abs(logprob.double().cpu().numpy() + np.log(n)) <= 2.0 ** -21 * (np.log(n) + 4)).all()
+    # 1 / (1e-6 + 1e-30) = 1e6 scales the gaps of the logits past what the noise spans (a gap of 1e-4 is 100)
+    top = x.topk(2, dim=1).values
+    clear = top[:, 0] - top[:, 1] > 1e-4
+    token, _ = fh.logits.choose(z, rules, temperature=1e-30, gumbel=g)
+    assert clear.any() and torch.equal(token.long()[clear], x.argmax(1)[clear])
 
 
 @pytest.mark.parametrize("V", [40, 3000, 33000])

@@ -78,7 +78,7 @@ def test_struct_layouts_match_the_header(tmp_path):
     (dict(out_dtype=_lib.FRL_ELT_F16), _lib.FRL_EINVAL), (dict(vocab=0), _lib.FRL_EINVAL), (dict(rows=-1), _lib.FRL_EINVAL),
     (dict(history_len=-1), _lib.FRL_EINVAL), (dict(n_sparse=-1), _lib.FRL_EINVAL), (dict(n_sparse=2049), _lib.FRL_EUNSUPPORTED),
     (dict(mask=3), _lib.FRL_EINVAL), (dict(vocab=(1 << 30) + 1, logits_stride=1 << 31, out_stride=1 << 31), _lib.FRL_EUNSUPPORTED),
-    (dict(rows=1 << 40), _lib.FRL_EUNSUPPORTED), (dict(logits_stride=31999), _lib.FRL_EINVAL), (dict(out_stride=31999), _lib.FRL_EINVAL),
+    (dict(rows=1 << 40), _lib.FRL_EUNSUPPORTED), (dict(n_sparse=4, history_len=1 << 19), _lib.FRL_EUNSUPPORTED), (dict(logits_stride=31999), _lib.FRL_EINVAL), (dict(out_stride=31999), _lib.FRL_EINVAL),
     (dict(history_len=4), _lib.FRL_EINVAL), (dict(n_sparse=4), _lib.FRL_EINVAL), (dict(mask=1), _lib.FRL_EINVAL),
 ])
 def test_constrain_refuses(lib, kw, code):
@@ -118,7 +118,7 @@ def test_choose_refuses(lib):
 @pytest.mark.parametrize("kw,code", [
     (dict(abi_version=5), _lib.FRL_EINVAL), (dict(dtype=3), _lib.FRL_EINVAL), (dict(teacher_dtype=-1), _lib.FRL_EINVAL), (dict(kind=2), _lib.FRL_EINVAL),
     (dict(reduction=3), _lib.FRL_EINVAL), (dict(rows=-1), _lib.FRL_EINVAL), (dict(vocab=0), _lib.FRL_EINVAL), (dict(top=0), _lib.FRL_EINVAL),
-    (dict(top=1025), _lib.FRL_EUNSUPPORTED), (dict(temperature=0.0), _lib.FRL_EINVAL), (dict(temperature=float("nan")), _lib.FRL_EINVAL),
+    (dict(top=1025), _lib.FRL_EUNSUPPORTED), (dict(temperature=0.0), _lib.FRL_EINVAL), (dict(temperature=float("nan")), _lib.FRL_EINVAL), (dict(temperature=float("inf")), _lib.FRL_EINVAL), (dict(temperature=1e-38), _lib.FRL_EINVAL),
     (dict(vocab=(1 << 30) + 1), _lib.FRL_EUNSUPPORTED), (dict(rows=(1 << 30) + 1), _lib.FRL_EUNSUPPORTED), (dict(logits_stride=31999), _lib.FRL_EINVAL),
     (dict(grad_stride=31999), _lib.FRL_EINVAL),
 ])
@@ -155,6 +155,10 @@ def test_host_tensors_and_wrong_arguments_are_refused():
         fh.logits.distill_loss(z, torch.zeros((2, 1), dtype=torch.int32), torch.zeros((2, 1)), reduction="batchmean")
     with pytest.raises(NotImplementedError, match="detach"):
         fh.logits.choose(torch.zeros((2, 8), requires_grad=True))
+    with pytest.raises(NotImplementedError, match="detach"):
+        fh.logits.choose(torch.zeros((2, 8)), temperature=torch.ones(2, requires_grad=True))
+    with pytest.raises(NotImplementedError, match="detach"):
+        fh.logits.constrain(torch.zeros((2, 8)), fh.logits.Constraints(repetition=torch.ones(2, requires_grad=True)))
 
 
 def test_marshalling_refuses_shapes_and_types():
