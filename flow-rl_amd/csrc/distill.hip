@@ -39,14 +39,32 @@ __device__ __forceinline__ float teacher_at(const void* p, long long i, int dtyp
   return Elt<F16>::get(((const F16*)p)[i]);
 }
 
-// the named tokens of [v0, v0 + n) as bits; `words` covers n rounded up to 32
+// n entries from z, cut where 16-byte vectors lie on 16-byte boundaries (rows of an odd two-byte vocabulary would otherwise read at odd
+// words: 171 against 138 us for a value of 2048 x 200001 bf16): `head` single entries, `nvec` vectors, `tail` single ones.  The entries' named bits
+// stand `pad` behind their number, so that a vector's bits do not cross a word.
+template <typename T>
+struct Cut {
+  static constexpr int N = Vec16<T>::N;
+  int head, nvec, tail, pad;
+  __device__ __forceinline__ Cut(const T* z, int n) {
+    head = min((N - (int)(((uintptr_t)z & 15) / sizeof(T))) % N, n);
+    nvec = (n - head) / N;
+    tail = n - head - nvec * N;
+    pad = (N - head) % N;
+  }
+  // the single entry that thread tid sees to, or -1 (G >= 16 threads: N for the head, N for the tail)
+  __device__ __forceinline__ int lone(int tid) const { return tid < head ? tid : tid >= N && tid - N < tail ? head + nvec * N + tid - N : -1; }
+  __device__ __forceinline__ int bit(int at) const { return head + pad + at * N; }
+};
+
+// the named tokens of [v0, v0 + n) as bits, token v0 at bit `pad`; `words` covers n rounded up to 32, and one more
 template <int G>
-__device__ __forceinline__ void mark_named(const DistillArgs& a, long long row, int tid, int v0, int n, unsigned* words) {
-  for (int w = tid; w < (n + 31) / 32; w += G) words[w] = 0u;
+__device__ __forceinline__ void mark_named(const DistillArgs& a, long long row, int tid, int v0, int n, int pad, unsigned* words) {
+  for (int w = tid; w < (n + 31) / 32 + 1; w += G) words[w] = 0u;
   group_sync<G>();
   for (int k = tid; k < a.top; k += G) {
     const long long loc = ld_id(a.ids, row * a.ids_stride + k, a.ids64) - v0;
-    if (loc >= 0 && loc < n) atomicOr(&words[loc >> 5], 1u << (loc & 31));
+    if (loc >= 0 && loc < n) atomicOr(&words[(loc + pad) >> 5], 1u << ((loc + pad) & 31));
   }
   group_sync<G>();
 }
@@ -80,9 +98,9 @@ struct Running {
       m = to;
     }
   }
-  // vectors [from, to) of z, G threads apart
+  // vectors [from, to) of the vectors at z, G threads apart; the first one's named bits begin at bit0
   template <typename T, int G>
-  __device__ __forceinline__ void stream(const T* z, int from, int to, float c, const unsigned* words, int tid) {
+  __device__ __forceinline__ void stream(const T* z, int from, int to, float c, const unsigned* words, int bit0, int tid) {
     constexpr int U = 4, N = Vec16<T>::N;
     for (int at = from + tid; at < to; at += U * G) {
       u32x4 raw[U];
@@ -105,7 +123,7 @@ struct Running {
         const float e = sum_of<N>(x);
         s += e;
         if constexpr (REST) {
-          const unsigned named = at + u * G < to ? named_bits<N>(words, (at + u * G) * N) : 0u;
+          const unsigned named = at + u * G < to ? named_bits<N>(words, bit0 + (at + u * G) * N) : 0u;
           r += named == 0u ? e : sum_unnamed<N>(x, named);
         }
       }
@@ -255,10 +273,10 @@ __device__ __forceinline__ void stream_gradient(const T* z, T* g, int from, int 
     u32x4 raw[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (at + u * G < to) raw[u] = ldu<u32x4>(z + (size_t)(at + u * G) * N);
+      if (at + u * G < to) raw[u] = ldu_nt<u32x4>(z + (size_t)(at + u * G) * N);
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (at + u * G < to) stu(g + (size_t)(at + u * G) * N, sc.of(raw[u]));
+      if (at + u * G < to) stu_nt(g + (size_t)(at + u * G) * N, sc.of(raw[u]));
   }
 }
 
@@ -297,17 +315,19 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, 4) frl_distill_row_kernel(c
   __shared__ float red0[WAVES], red1[WAVES];
   __shared__ double row_p[GPB], row_x[GPB];
   const int tid = threadIdx.x % G, grp = G < 64 ? threadIdx.x / G : G == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
-  const int nwords = REST ? (a.vocab + 31) / 32 : 0;
+  const int nwords = REST ? (a.vocab + 31) / 32 + 1 : 0;
   unsigned* words = lds + (size_t)grp * (nwords + 3 * a.top);
   int* sid = (int*)(words + nwords);
   float* sp = (float*)(sid + a.top);
   float* sz = sp + a.top;
   const float inv = a.inv_denom != nullptr ? *a.inv_denom : a.denom_scale;
-  const int nvec = a.vocab / N, tail = a.vocab - nvec * N, nv = (nvec + G - 1) / G;
   const long long row = block_index() * GPB + grp;
   if (row >= a.rows) return;
   const T* z = (const T*)a.logits + row * a.logits_stride;
   T* g = GRAD ? (T*)a.grad + row * a.grad_stride : nullptr;
+  const Cut<T> cut(z, a.vocab);
+  const T* zv = z + cut.head;
+  const int nvec = cut.nvec, nv = (nvec + G - 1) / G, lone = cut.lone(tid);
   const float w = a.weights != nullptr ? a.weights[row] : 1.0f;
   if (w == 0.0f) {                                       // uniform over the group
     if (tid == 0) {
@@ -324,17 +344,17 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, 4) frl_distill_row_kernel(c
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     raw[i] = Vec16<T>::fill_minus_inf();
-    if (i < nv && i * G + t0 < nvec) raw[i] = ldu<u32x4>((const char*)z + 16u * (unsigned)(i * G + t0));
+    if (i < nv && i * G + t0 < nvec) raw[i] = ldu_nt<u32x4>((const char*)zv + 16u * (unsigned)(i * G + t0));
   }
-  if constexpr (REST) mark_named<G>(a, row, tid, 0, a.vocab, words);
+  if constexpr (REST) mark_named<G>(a, row, tid, 0, a.vocab, cut.pad, words);
   if (tid < 64) {
     double sum_p, cross;
     teacher_part<T, G < 64 ? G : 64, REST>(a, row, z, tid, sid, sp, sz, sum_p, cross);
     if (tid == 0) { row_p[grp] = sum_p; row_x[grp] = cross; }
   }
   Running<REST> run;
-  if (nvec > NV * G) run.template stream<T, G>(z, NV * G, nvec, a.scale2, words, t0);
-  if (tid < tail) run.one(Elt<T>::get(z[nvec * N + tid]), a.scale2, REST && named_bits<1>(words, nvec * N + tid) != 0u);
+  if (nvec > NV * G) run.template stream<T, G>(zv, NV * G, nvec, a.scale2, words, cut.bit(0), t0);
+  if (lone >= 0) run.one(Elt<T>::get(z[lone]), a.scale2, REST && named_bits<1>(words, lone + cut.pad) != 0u);
   float m = run.m;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
@@ -358,7 +378,7 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, 4) frl_distill_row_kernel(c
       const float e = sum_of<N>(x);
       run.s += e;
       if constexpr (REST) {
-        const unsigned named = i * G + t1 < nvec ? named_bits<N>(words, (i * G + t1) * N) : 0u;
+        const unsigned named = i * G + t1 < nvec ? named_bits<N>(words, cut.bit(i * G + t1)) : 0u;
         run.r += named == 0u ? e : sum_unnamed<N>(x, named);
       }
       __builtin_amdgcn_sched_barrier(0);                     // one vector unpacked at a time: eight independent elements are parallel enough
@@ -379,11 +399,11 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, 4) frl_distill_row_kernel(c
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if (i < nv && i * G + t2 < nvec) {
-          stu((char*)g + 16u * (unsigned)(i * G + t2), sc.of(raw[i]));
+          stu_nt((char*)(g + cut.head) + 16u * (unsigned)(i * G + t2), sc.of(raw[i]));
           __builtin_amdgcn_sched_barrier(0);
         }
-      if (nvec > NV * G) stream_gradient<T, G>(z, g, NV * G, nvec, sc, t2);
-      if (tid < tail) g[nvec * N + tid] = Elt<T>::put(sc.one(Elt<T>::get(z[nvec * N + tid])));
+      if (nvec > NV * G) stream_gradient<T, G>(zv, g + cut.head, NV * G, nvec, sc, t2);
+      if (lone >= 0) g[lone] = Elt<T>::put(sc.one(Elt<T>::get(z[lone])));
       group_sync<G>();
       named_gradient<T, G>(a, g, 0, a.vocab, sh, f * k.k_named * k.inv_s, f, sid, sp, sz, tid);
     }
@@ -405,13 +425,14 @@ __global__ void __launch_bounds__(G) frl_distill_part_kernel(const DistillArgs a
   const long long row = item / a.segs;
   const int v0 = (int)(item - row * a.segs) * a.seg_len, n = min(a.vocab - v0, a.seg_len);
   if (a.weights != nullptr && a.weights[row] == 0.0f) return;
-  if constexpr (REST) mark_named<G>(a, row, threadIdx.x, v0, n, lds);
-  const T* z = (const T*)a.logits + row * a.logits_stride + v0;
-  constexpr int N = Vec16<T>::N;
-  const int nvec = n / N, tid = threadIdx.x;
+    const T* z = (const T*)a.logits + row * a.logits_stride + v0;
+  const int tid = threadIdx.x;
+  const Cut<T> cut(z, n);
+  const int lone = cut.lone(tid);
+  if constexpr (REST) mark_named<G>(a, row, tid, v0, n, cut.pad, lds);
   Running<REST> run;
-  run.template stream<T, G>(z, 0, nvec, a.scale2, lds, tid);
-  if (tid < n - nvec * N) run.one(Elt<T>::get(z[nvec * N + tid]), a.scale2, REST && named_bits<1>(lds, nvec * N + tid) != 0u);
+  run.template stream<T, G>(z + cut.head, 0, cut.nvec, a.scale2, lds, cut.bit(0), tid);
+  if (lone >= 0) run.one(Elt<T>::get(z[lone]), a.scale2, REST && named_bits<1>(lds, lone + cut.pad) != 0u);
   const float m = group_reduce<MaxOp, G>(run.m, red0);
   run.about(m, a.scale2);
   const float s = group_reduce<SumOp, G>(run.s, red1), r = REST ? group_reduce<SumOp, G>(run.r, red0) : 0.0f;   // red0: read before the barrier in the sum
@@ -502,9 +523,10 @@ __global__ void __launch_bounds__(G == 64 ? 256 : G) frl_distill_grad_kernel(con
   const float f = cot * w * inv * a.inv_temp;
   const Shift sh(st[0], a.scale2);
   const Scaled<T> sc(sh, f * st[3] * st[1]);
-  const int nvec = n / N, tail = n - nvec * N;
-  stream_gradient<T, G>(z + v0, g + v0, 0, nvec, sc, tid);
-  if (tid < tail) g[v0 + nvec * N + tid] = Elt<T>::put(sc.one(Elt<T>::get(z[v0 + nvec * N + tid])));
+  const Cut<T> cut(z + v0, n);
+  const int lone = cut.lone(tid);
+  stream_gradient<T, G>(z + v0 + cut.head, g + v0 + cut.head, 0, cut.nvec, sc, tid);
+  if (lone >= 0) g[v0 + lone] = Elt<T>::put(sc.one(Elt<T>::get(z[v0 + lone])));
   if (tid < 64) {
     double sum_p, cross;
     teacher_part<T, 64, REST>(a, row, z, tid, sid, sp, sz, sum_p, cross);
@@ -641,7 +663,7 @@ static DistillWs distill_ws(const FrlDistillDesc* d, const DistillPlan& p) {
 
 template <typename T, bool REST>
 static hipError_t launch_rows(const DistillArgs& a, const DistillPlan& p, bool grad, hipStream_t st) {
-  const size_t per = ((size_t)(REST ? (a.vocab + 31) / 32 : 0) + 3 * (size_t)a.top) * 4;
+  const size_t per = ((size_t)(REST ? (a.vocab + 31) / 32 + 1 : 0) + 3 * (size_t)a.top) * 4;
   const int gpb = p.G <= 64 ? 256 / p.G : 1;
   const size_t lds = gpb * per;
   const long long blocks = (a.rows + gpb - 1) / gpb;
@@ -672,7 +694,7 @@ static hipError_t launch_rows(const DistillArgs& a, const DistillPlan& p, bool g
 template <typename T, bool REST>
 static hipError_t launch_parts(const DistillArgs& a, float* loss, float* inv, hipStream_t st) {
   const long long items = a.rows * a.segs;
-  hipLaunchKernelGGL((frl_distill_part_kernel<T, 256, REST>), grid_of(items), dim3(256), REST ? (size_t)((a.seg_len + 31) / 32) * 4 : 0, st, a);
+  hipLaunchKernelGGL((frl_distill_part_kernel<T, 256, REST>), grid_of(items), dim3(256), REST ? (size_t)((a.seg_len + 31) / 32 + 1) * 4 : 0, st, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const int waves = loss != nullptr ? (int)a.rows : 1;

@@ -30,6 +30,18 @@ __device__ __forceinline__ void stu(void* p, V v) {
   __builtin_memcpy(p, &v, sizeof(V));
 }
 
+// The same with the non-temporal hint, for what is read once or written once: it leaves the caches first, and what is read again stays
+template <typename V>
+__device__ __forceinline__ void stu_nt(void* p, V v) {
+  typedef V VU __attribute__((aligned(2)));
+  __builtin_nontemporal_store(v, (VU*)p);
+}
+template <typename V>
+__device__ __forceinline__ V ldu_nt(const void* p) {
+  typedef V VU __attribute__((aligned(2)));
+  return __builtin_nontemporal_load((const VU*)p);
+}
+
 struct Bf16 { unsigned short u; };
 struct F16 { unsigned short u; };
 
@@ -39,7 +51,7 @@ template <> struct Elt<float> {
   static __device__ __forceinline__ float get(float v) { return v; }
   static __device__ __forceinline__ float put(float v) { return v; }
   static __device__ __forceinline__ f32x4 load4(const float* p) { return ldu<f32x4>(p); }
-  static __device__ __forceinline__ void store4(float* p, f32x4 v) { stu(p, v); }
+  static __device__ __forceinline__ void store4(float* p, f32x4 v) { stu_nt(p, v); }
 };
 template <> struct Elt<Bf16> {
   static constexpr int id = FRL_ELT_BF16;
@@ -49,7 +61,7 @@ template <> struct Elt<Bf16> {
     const u32x2 r = ldu<u32x2>(p);
     return f32x4{__uint_as_float(r[0] << 16), __uint_as_float(r[0] & 0xffff0000u), __uint_as_float(r[1] << 16), __uint_as_float(r[1] & 0xffff0000u)};
   }
-  static __device__ __forceinline__ void store4(Bf16* p, f32x4 v) { stu(p, u16x4{put(v[0]).u, put(v[1]).u, put(v[2]).u, put(v[3]).u}); }
+  static __device__ __forceinline__ void store4(Bf16* p, f32x4 v) { stu_nt(p, u16x4{put(v[0]).u, put(v[1]).u, put(v[2]).u, put(v[3]).u}); }
 };
 template <> struct Elt<F16> {
   static constexpr int id = FRL_ELT_F16;
@@ -59,7 +71,7 @@ template <> struct Elt<F16> {
     const u16x4 r = ldu<u16x4>(p);
     return f32x4{get(F16{r[0]}), get(F16{r[1]}), get(F16{r[2]}), get(F16{r[3]})};
   }
-  static __device__ __forceinline__ void store4(F16* p, f32x4 v) { stu(p, u16x4{put(v[0]).u, put(v[1]).u, put(v[2]).u, put(v[3]).u}); }
+  static __device__ __forceinline__ void store4(F16* p, f32x4 v) { stu_nt(p, u16x4{put(v[0]).u, put(v[1]).u, put(v[2]).u, put(v[3]).u}); }
 };
 
 // 16 bytes of a row at a time: VEC elements, kept packed until they are used

@@ -168,7 +168,7 @@ template <typename T>
 struct Packed4 {
   u32x2 r;
   __device__ __forceinline__ void load(const T* p, int left) {
-    if (left >= 4) { r = ldu<u32x2>(p); return; }
+    if (left >= 4) { r = ldu_nt<u32x2>(p); return; }
     const unsigned ninf = Elt<T>::put(-INFINITY).u;
     const unsigned e0 = left > 0 ? p[0].u : ninf, e1 = left > 1 ? p[1].u : ninf, e2 = left > 2 ? p[2].u : ninf;
     r = u32x2{e0 | e1 << 16, e2 | ninf << 16};
@@ -182,7 +182,7 @@ struct Packed4 {
 template <>
 struct Packed4<float> {
   f32x4 r;
-  __device__ __forceinline__ void load(const float* p, int left) { r = load_quad(p, left, -INFINITY); }
+  __device__ __forceinline__ void load(const float* p, int left) { r = left >= 4 ? ldu_nt<f32x4>(p) : load_quad(p, left, -INFINITY); }
   __device__ __forceinline__ void none() { r = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY}; }
   __device__ __forceinline__ f32x4 get() const { return r; }
 };

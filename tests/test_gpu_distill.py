@@ -179,18 +179,31 @@ def test_strides_types_and_leading_dimensions():
     import torch
     import flowrl_hip as fh
     rng = np.random.default_rng(2)
-    for N, V, K in ((6, 77, 9), (3, 2501, 40), (4, 20003, 5)):
-        z, ids, t = make_distill(rng, N, V, K, "logits", torch.bfloat16, ragged=True)
+    for N, V, K in ((6, 77, 9), (3, 2501, 40), (4, 20003, 5), (300, 9001, 20)):
+        z, ids, t = make_distill(rng, N, V, K, "logprobs", torch.bfloat16, ragged=True)
         zc, ic, tc = z.cuda(), torch.from_numpy(ids).cuda(), torch.from_numpy(t).cuda()
-        want = fh.logits.distill_loss(zc, ic, tc, want_grad=True)
-        buf = torch.zeros((N * (V + 3) + 1,), dtype=torch.bfloat16, device="cuda")
-        view = buf[1:].view(N, V + 3)[:, :V]
-        view.copy_(zc)
-        same = [(view, ic, tc), (zc, ic.long(), tc), (zc.t().contiguous().t(), ic.t().contiguous().t(), tc.t().contiguous().t()),
+        kw = dict(kind="logprobs", want_grad=True)
+        want = fh.logits.distill_loss(zc, ic, tc, **kw)
+        same = [(zc, ic.long(), tc), (zc.t().contiguous().t(), ic.t().contiguous().t(), tc.t().contiguous().t()),
                 (zc, torch.cat([ic, ic], 1)[:, :K], torch.cat([tc, tc], 1)[:, :K])]
         for a in same:
-            got = fh.logits.distill_loss(*a, want_grad=True)
+            got = fh.logits.distill_loss(*a, **kw)
             assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        # where a row starts decides how it is cut into vectors, so the order of its sum: against the formula
+        L, g, tolL, tolg = _expected(z, ids, t, "logprobs", 1.0)
+        for skip, gap in ((1, 3), (3, 0), (7, 8), (2, 1)):
+            buf = torch.zeros((N * (V + gap) + skip,), dtype=torch.bfloat16, device="cuda")
+            view = buf[skip:].view(N, V + gap)[:, :V]
+            view.copy_(zc)
+            loss, grad = fh.logits.distill_loss(view, ic, tc, **kw)
+            assert abs(float(loss) - L.mean()) <= tolL.max() + 2.0 ** -24 * abs(L.mean())
+            _close(grad, g, tolg, 1.0 / N)
+            rows = fh.logits.distill_loss(view, ic, tc, kind="logprobs", reduction="none").double().cpu().numpy()
+            assert (np.abs(rows - L) <= tolL).all()
+            leaf = view.detach().requires_grad_(True)
+            got, = torch.autograd.grad(fh.autograd.distill_loss(leaf, ic, tc, kind="logprobs"), leaf)
+            _close(got, g, tolg, 1.0 / N)
+        tc = torch.from_numpy(t - t.max() - 1).cuda()
         for dt in (torch.bfloat16, torch.float16):
             narrow = tc.to(dt)
             a, b = fh.logits.distill_loss(zc, ic, narrow), fh.logits.distill_loss(zc, ic, narrow.float())
