@@ -7,11 +7,13 @@
 //     dL/dz  = k q / T            the others, k = 1 (FRL_DISTILL_TOP) or 1 - P s / r (FRL_DISTILL_REST with P > 0)
 // The gradient is therefore one scaled exponential per element plus a correction of `top` elements.
 //
-// HBM-bound for long rows: the logits once, the gradient once.  A row lives in the registers of the threads that share it (a wave up to a
-// workgroup of 1024, at most 16 vectors of 16 bytes each: 131072 entries of two bytes), so the gradient needs no second read.  With q
-// bounded by quarter-rate exponentials (four issue slots each) the rest of the arithmetic is kept to four slots per element: the shift
-// by the maximum is one fma, two bytes are packed by one convert, and the factor of a two-byte gradient goes into the exponent.
-// Rows beyond that, or too few to fill the chip, are split over their length, joined by a second kernel, and differentiated by a third.
+// HBM-bound for long rows: the logits once, the gradient once.  For a gradient a row lives in the registers of the threads that share it (16
+// lanes up to a workgroup of 512, at most 16 vectors of 16 bytes each: 65536 entries of two bytes) and behind those in LDS (36864 more); only what
+// is longer is read a second time.  A value keeps nothing and streams.  An element costs two quarter-rate exponentials (four issue slots each), one
+// for the sum and one for the gradient; the rest is kept to four slots per element: the shift by the maximum is one fma, two bytes are packed by one
+// convert, and the factor of a two-byte gradient goes into the exponent.  The gradient, and logits that are read for the last time, pass the
+// caches by (non-temporal): 8192 x 131072 bf16 with its gradient 963 -> 907 us, 4096 x 32000 126 -> 107.
+// Rows beyond 2^18 entries, or too few to fill the chip, are split over their length, joined by a second kernel, and differentiated by a third.
 #include "frl_rows.h"
 
 namespace frl {
@@ -27,6 +29,7 @@ struct DistillArgs {
   long long rows, logits_stride, grad_stride, ids_stride, teacher_stride;
   float inv_temp, scale2, denom_scale;   // 1 / T, log2(e) / T
   int vocab, top, ids64, teacher_dtype, segs, seg_len, g_stride;
+  int kept, kept_at;          // row kernel: vectors per thread that stay in LDS behind those in registers, and where (in words)
 };
 
 constexpr double LN2 = 0.6931471805599453;
@@ -98,14 +101,20 @@ struct Running {
       m = to;
     }
   }
-  // vectors [from, to) of the vectors at z, G threads apart; the first one's named bits begin at bit0
+  // vectors [from, to) of the vectors at z, G threads apart; the first one's named bits begin at bit0.  Those before `keep` stay in LDS (at `kept`) for
+  // the same thread's gradient.
   template <typename T, int G>
-  __device__ __forceinline__ void stream(const T* z, int from, int to, float c, const unsigned* words, int bit0, int tid) {
+  __device__ __forceinline__ void stream(const T* z, int from, int to, float c, const unsigned* words, int bit0, int tid, int keep = 0, u32x4* kept = nullptr) {
     constexpr int U = 4, N = Vec16<T>::N;
     for (int at = from + tid; at < to; at += U * G) {
       u32x4 raw[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) raw[u] = at + u * G < to ? ldu<u32x4>(z + (size_t)(at + u * G) * N) : Vec16<T>::fill_minus_inf();
+      if (keep > 0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (at + u * G < keep) kept[at + u * G - from] = raw[u];
+      }
       float bm = m;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -267,8 +276,12 @@ struct Scaled {
 };
 
 template <typename T, int G>
-__device__ __forceinline__ void stream_gradient(const T* z, T* g, int from, int to, const Scaled<T>& sc, int tid) {
+__device__ __forceinline__ void stream_gradient(const T* z, T* g, int from, int to, const Scaled<T>& sc, int tid, int keep = 0, const u32x4* kept = nullptr) {
   constexpr int U = 4, N = Vec16<T>::N;
+  int done = from;
+  for (; done < keep; done += G)                           // what the sums left in LDS
+    if (done + tid < min(keep, to)) stu_nt(g + (size_t)(done + tid) * N, sc.of(kept[done + tid - from]));
+  from = done;
   for (int at = from + tid; at < to; at += U * G) {
     u32x4 raw[U];
 #pragma unroll
@@ -307,6 +320,9 @@ __device__ __forceinline__ void keep_packed(u32x4* raw) {
 }
 
 // A row to a group, its first NV vectors per thread held in registers: value, what the backward needs, and (GRAD) the gradient.
+// Bound by HBM: 2048 x 131072 bf16, value: 92 us, 5.8 TB/s of the 5.9 that reads alone reach; 4096 x 32000 bf16 with its gradient: 100 us, 5.2 TB/s;
+// 8192 x 131072 bf16 with named rest and gradient: 885 us, 4.9 TB/s (a large copy: 4.9 to 5.4).  A row's passes (maximum, sum, gradient) wait for
+// one another, so it takes a second workgroup on the CU to keep the memory busy; hence at most 512 threads with what they hold in registers.
 template <typename T, int G, int NV, bool REST, bool GRAD>
 __global__ void __launch_bounds__(G <= 64 ? 256 : G, 4) frl_distill_row_kernel(const DistillArgs a) {
   extern __shared__ __align__(16) unsigned lds[];
@@ -320,6 +336,7 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, 4) frl_distill_row_kernel(c
   int* sid = (int*)(words + nwords);
   float* sp = (float*)(sid + a.top);
   float* sz = sp + a.top;
+  u32x4* kept = (u32x4*)(lds + a.kept_at);
   const float inv = a.inv_denom != nullptr ? *a.inv_denom : a.denom_scale;
   const long long row = block_index() * GPB + grp;
   if (row >= a.rows) return;
@@ -353,7 +370,7 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, 4) frl_distill_row_kernel(c
     if (tid == 0) { row_p[grp] = sum_p; row_x[grp] = cross; }
   }
   Running<REST> run;
-  if (nvec > NV * G) run.template stream<T, G>(zv, NV * G, nvec, a.scale2, words, cut.bit(0), t0);
+  if (nvec > NV * G) run.template stream<T, G>(zv, NV * G, nvec, a.scale2, words, cut.bit(0), t0, GRAD ? (NV + a.kept) * G : 0, kept);
   if (lone >= 0) run.one(Elt<T>::get(z[lone]), a.scale2, REST && named_bits<1>(words, lone + cut.pad) != 0u);
   float m = run.m;
 #pragma unroll
@@ -402,7 +419,7 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, 4) frl_distill_row_kernel(c
           stu_nt((char*)(g + cut.head) + 16u * (unsigned)(i * G + t2), sc.of(raw[i]));
           __builtin_amdgcn_sched_barrier(0);
         }
-      if (nvec > NV * G) stream_gradient<T, G>(zv, g + cut.head, NV * G, nvec, sc, t2);
+      if (nvec > NV * G) stream_gradient<T, G>(zv, g + cut.head, NV * G, nvec, sc, t2, (NV + a.kept) * G, kept);
       if (lone >= 0) g[lone] = Elt<T>::put(sc.one(Elt<T>::get(z[lone])));
       group_sync<G>();
       named_gradient<T, G>(a, g, 0, a.vocab, sh, f * k.k_named * k.inv_s, f, sid, sp, sz, tid);
@@ -425,7 +442,7 @@ __global__ void __launch_bounds__(G) frl_distill_part_kernel(const DistillArgs a
   const long long row = item / a.segs;
   const int v0 = (int)(item - row * a.segs) * a.seg_len, n = min(a.vocab - v0, a.seg_len);
   if (a.weights != nullptr && a.weights[row] == 0.0f) return;
-    const T* z = (const T*)a.logits + row * a.logits_stride + v0;
+  const T* z = (const T*)a.logits + row * a.logits_stride + v0;
   const int tid = threadIdx.x;
   const Cut<T> cut(z, n);
   const int lone = cut.lone(tid);
@@ -583,11 +600,12 @@ __global__ void __launch_bounds__(1024) frl_distill_sum_kernel(const float* __re
 
 struct DistillPlan { int G, NV, segs, seg_len; bool split; };
 
-// Threads per row: 16 lanes for a row of at most 256 entries and 64 names, else as few as hold it with 16 vectors of 16 bytes each, more while the rows alone leave the chip's 1024 SIMDs short of four
-// waves.  A value alone keeps nothing and streams, up to 1024 threads; a gradient keeps what 512 threads hold (two workgroups to a CU, one
-// loads while the other computes) and reads the rest of a longer row again.  Measured, bf16, value + gradient: 8192 x 131072 990 us so, 1127
-// with 1024 threads and all of it held, 1158 with nothing held; 4096 x 32000 130 with 256 threads, 157 with 512; 2048 x 131072, value alone:
-// 95 us streamed by 1024 threads, 115 held by 512.
+// Threads per row: 16 lanes for a row of at most 256 entries and 64 names (65536 x 200 f32 with gradient: 42 us so, 69 by a wave), else as few as hold
+// it with 16 vectors of 16 bytes each, more while the rows alone leave the chip's 1024 SIMDs short of four waves.  A value alone keeps nothing and
+// streams, up to 1024 threads; a gradient keeps what 512 threads hold (two workgroups to a CU, one loads while the other computes) and reads what
+// LDS does not hold of a longer row again.  Measured, bf16, value + gradient: 8192 x 131072 920 us by 512 threads with 16 vectors each, 1145 by 1024
+// threads and all of it held, 968 by 512 with nothing held; 4096 x 32000 109 by 256 threads, 133 by 512.  2048 x 131072, value alone: 95 us streamed
+// by 1024 threads, 115 held by 512.
 // Fewer than 256 rows of more than 8192 entries, and rows whose named bits would take more than 32 KB of LDS, are split: at least 512 segments,
 // each of 4096 to 65536 entries.
 static DistillPlan distill_plan(const FrlDistillDesc* d, bool grad) {
@@ -662,10 +680,19 @@ static DistillWs distill_ws(const FrlDistillDesc* d, const DistillPlan& p) {
 }
 
 template <typename T, bool REST>
-static hipError_t launch_rows(const DistillArgs& a, const DistillPlan& p, bool grad, hipStream_t st) {
+static hipError_t launch_rows(DistillArgs a, const DistillPlan& p, bool grad, hipStream_t st) {
   const size_t per = ((size_t)(REST ? (a.vocab + 31) / 32 + 1 : 0) + 3 * (size_t)a.top) * 4;
   const int gpb = p.G <= 64 ? 256 / p.G : 1;
-  const size_t lds = gpb * per;
+  size_t lds = gpb * per;
+  if (grad && p.G == 512 && a.vocab > p.G * p.NV * Vec16<T>::N) {
+    // Two workgroups to a CU's 160 KB: what is left of a half, 9 vectors a thread and fewer beside named bits, holds more of the row (512 bytes are the
+    // kernel's own arrays).  Measured, bf16, against reading that part again: 8192 x 131072 913 -> 896 us, 2048 x 200000 343 -> 334.
+    constexpr size_t HALF = 80 * 1024 - 512;
+    lds = (lds + 15) / 16 * 16;
+    a.kept_at = (int)(lds / 4);
+    a.kept = (int)((HALF - lds) / ((size_t)p.G * 16));
+    lds += (size_t)a.kept * p.G * 16;
+  }
   const long long blocks = (a.rows + gpb - 1) / gpb;
   const dim3 grid = grid_of(blocks);
 #define FRL_GO(g, nv, gr) hipLaunchKernelGGL((frl_distill_row_kernel<T, g, nv, REST, gr>), grid, dim3(g <= 64 ? 256 : g), lds, st, a)

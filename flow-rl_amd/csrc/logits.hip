@@ -423,8 +423,9 @@ struct LogitsPlan { int G, chunks, per, parts; };
 
 // Threads per chunk: a wave for short rows; a workgroup of 1024 where lists have to be searched for every chunk and the batch gives every CU two such
 // workgroups; else 256.  A group takes so many chunks of a row that about one round (1024 threads) or two (256) of resident groups remain.  Measured,
-// bf16 choice of 256 x 131072: with a history of 4096, 68 us by 1024 threads in 512 groups, 75 in 1024 groups, 90 by 256 threads in 4096;
-// without lists 39 us by 1024 threads, 37.5 by 256.
+// choice of 256 x 131072 bf16: with a history of 4096, 43 us by 1024 threads in 512 groups, 49 in 1024 groups, 64 by 256 threads; without lists 30 by
+// 1024 threads, 29 by 256.  Constraining 512 x 131072 f32 with a history of 4096: 106 by 1024 threads, 144 by 256; 4096 x 4000 bf16 with a history of
+// 1000: 22 by 256 threads, 37 by 1024; 512 x 131072 f32 with a mask alone: 101 in two rounds, 107 in one.
 static LogitsPlan logits_plan(const FrlLogitsDesc* d) {
   LogitsPlan p;
   const long long wide = d->rows * (((long long)d->vocab + 8191) / 8192);
