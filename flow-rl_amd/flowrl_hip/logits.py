@@ -242,10 +242,11 @@ def constrain(logits: torch.Tensor, rules: Optional[Constraints] = None, *, out:
     tensor of the logits' shape with contiguous rows; it may be ``logits`` itself."""
     rules = _NO_RULES if rules is None else rules
     if torch.is_grad_enabled():
-        _no_grad("logits / a rule", logits, *_differentiable(rules))
+        _no_grad("logits / a rule / out", logits, out, *_differentiable(rules))
     z, R, V, stride = _check_logits(logits, "logits")
     index = logits.get_device()
-    if out is None:
+    given = out is not None
+    if not given:
         dtype = logits.dtype if out_dtype is None else out_dtype
         out = torch.empty_like(logits, dtype=dtype, memory_format=torch.contiguous_format)
         o_stride = V
@@ -265,6 +266,8 @@ def constrain(logits: torch.Tensor, rules: Optional[Constraints] = None, *, out:
         raise TypeError(f"constrain: {logits.dtype} logits go to {logits.dtype} or float32, not {dtype}")
     d, b, keep = _marshal(z, R, V, rules, stride, _ELT[dtype], o_stride, out.data_ptr())
     _call(_lib.load().frl_logits_constrain, index, C.byref(d), C.byref(b))
+    if given and not out.is_inference():
+        torch.autograd.graph.increment_version(out)        # written behind torch's back: a graph that saved it has to notice
     return out
 
 

@@ -338,3 +338,51 @@ def test_answer_teach_answer():
             L64, g64[r] = L64 + L, g
         assert abs(float(loss) - L64) <= R * 2.0 ** -17
         t64 = t64 - 0.5 * g64
+
+
+@pytest.mark.parametrize("kind", ["logits", "logprobs"])
+@pytest.mark.parametrize("V,dtype", [(32771, "float32"), (51207, "float32"), (60003, "float32"), (65543, "bfloat16"), (102417, "float16"), (140001, "bfloat16")])
+def test_rows_longer_than_registers(V, dtype, kind):
+    """A batch that is not split, of rows that registers hold but for a few entries, that LDS holds beside them, and that are read twice: named
+    entries at the ends of each, steep rows, a row of weight 0."""
+    import torch
+    import flowrl_hip as fh
+    rng = np.random.default_rng(V)
+    N, K, T, dt = 257, 12, 1.5, getattr(torch, dtype)
+    held = 32768 if dt == torch.float32 else 65536
+    z, ids, t = make_distill(rng, N, V, K, kind, dt)
+    ids[:, :6] = [0, V - 1, held - 1, held, held + 2, V - 9]
+    ids[:, 6:] = 100 + np.arange(6) * 1111
+    z[3, held:] += 20.0                            # the maximum lies behind what is held
+    z[4, :held] = float("-inf")
+    z[5, held:] = float("-inf")
+    zc, ic, tc = z.cuda(), torch.from_numpy(ids).cuda(), torch.from_numpy(t).cuda()
+    w = np.ones(N, np.float32)
+    w[6] = 0.0
+    wc = torch.from_numpy(w).cuda()
+    kw = dict(kind=kind, temperature=T, weights=wc, reduction="none")
+    rows, grad = fh.logits.distill_loss(zc, ic, tc, want_grad=True, **kw)
+    value = fh.logits.distill_loss(zc, ic, tc, **kw)
+    leaf = zc.clone().requires_grad_(True)
+    out = fh.autograd.distill_loss(leaf, ic, tc, **kw)
+    back, = torch.autograd.grad(out, leaf, torch.ones_like(out))
+    pick = [0, 1, 3, 128, 255, 256]
+    L, g, tolL, tolg = _expected(z[pick], ids[pick], t[pick], kind, T)
+    for got in (rows, value, out.detach()):
+        assert (np.abs(got[pick].double().cpu().numpy() - L) <= tolL).all()
+    for got in (grad, back):
+        _close(got[pick], g, tolg + np.abs(g) * 2.0 ** -22, 1.0)
+        assert not got[6].any()
+    assert rows[6] == 0.0 and value[6] == 0.0
+    for r in (4, 5):                               # -inf at a named entry: an infinite divergence, and gradients that stay numbers
+        assert rows[r] == float("inf") and value[r] == float("inf")
+        free = np.setdiff1d(np.flatnonzero(np.isneginf(z[r].float().numpy())), ids[r])
+        assert not grad[r].cpu()[free].any()
+    # every row against torch's float32 log sum exp (off by at most 2^-20 of itself and its largest argument, below 40 here)
+    lse = torch.logsumexp(zc.float() / T, 1)
+    assert torch.isfinite(lse).all()
+    if kind == "logits":
+        p = torch.softmax(tc.double() / T, 1)
+        want = (p * (p.log() + lse.double()[:, None] - zc.gather(1, ic.long()).double() / T)).sum(1) * wc
+        fine = torch.isfinite(want)
+        assert ((rows.double() - want)[fine].abs() <= 2.0 ** -16 * (want[fine].abs() + 40)).all()

@@ -83,6 +83,8 @@ CASES = [
     (2, 40, dict(hist=9, sparse=2048), "bool"),                             # lists far longer than the row
     (3, 70001, dict(hist=9000, prompt=True, sparse=600, wide=True), "bool"),   # a history that no group keeps in registers
     (560, 9001, dict(hist=5000, prompt=True), None),
+    (128, 70001, dict(hist=3000, prompt=True, sparse=50), "words"),         # several chunks to a workgroup of 1024 threads
+    (4300, 4001, dict(hist=50, sparse=5), "words"),                         # and to one of 256
 ]
 IDS = [f"{R}x{V}-{'-'.join(k for k in kw)}-{mask}" for R, V, kw, mask in CASES]
 
@@ -386,3 +388,21 @@ def test_critic_choice_with_candidates_ruled_out():
     everything = torch.ones((B, N), dtype=torch.bool, device="cuda")
     a, b = fh.critic_select(critic, p, obs, actions, N, allowed=everything), fh.critic_select(critic, p, obs, actions, N)
     assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_in_place_is_noticed_by_graphs():
+    """torch's graphs refuse a backward whose saved tensor `out=` has overwritten."""
+    import torch
+    import flowrl_hip as fh
+    z = torch.randn(3, 40, device="cuda")
+    s = torch.ones((), device="cuda", requires_grad=True)
+    y = (z * s).sum()                              # keeps z for the gradient of s
+    fh.logits.constrain(z, fh.logits.Constraints(bias=torch.ones(40, device="cuda")), out=z)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        q = torch.zeros(3, 40, device="cuda")
+        fh.logits.constrain(z, out=q)
+        assert torch.equal(q, z)
+    with pytest.raises(NotImplementedError):
+        fh.logits.constrain(z, out=torch.zeros(3, 40, device="cuda", requires_grad=True))
