@@ -88,7 +88,8 @@ def _distinct(gen, rows, count, vocab):
     u = torch.rand((rows, count), generator=gen, device="cuda", dtype=torch.float64)
     at = torch.arange(count, device="cuda", dtype=torch.float64)
     lo, hi = (at * vocab / count).ceil(), ((at + 1) * vocab / count).ceil()
-    ids = torch.minimum((lo + u * (hi - lo)).floor(), hi - 1).long()
+    # a device's quotient can be a rounding above vocab at the last end (32000 * 300 / 300), one token too many
+    ids = torch.minimum((lo + u * (hi - lo)).floor(), hi - 1).clamp_(max=vocab - 1).long()
     order = torch.rand((rows, count), generator=gen, device="cuda").argsort(dim=1)
     return ids.gather(1, order)
 
