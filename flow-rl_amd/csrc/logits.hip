@@ -4,12 +4,15 @@
 // its token stands in the row's history, then its biases, then the mask; choose adds y = x / T, key = y + gumbel, the first
 // argmax of key and y[token] - log sum exp y from a maximum and a sum.
 //
-// HBM-bound: an element is read once (and, choose, its noise), a result written once.  What must not cost a pass over the
+// HBM-bound where the lists are short: an element is read once (and, choose, its noise), a result written once.  What must not cost a pass over the
 // vocabulary of its own is the lists, a history of tokens and biases by token.  A group of G threads (a wave up to a workgroup of 1024) takes
 // consecutive chunks of 8 G entries of one row.  For each it counts the history's tokens that fall into the chunk in one LDS word per entry
 // (integer adds: any order gives the same counts), puts the number of a listed bias beside the count, and applies both to the
 // logits, which are on their way meanwhile.  Two sets of words take turns, so a chunk costs one barrier; a choice keeps its maximum and sum in
 // registers from chunk to chunk and reduces them once.
+// Measured: constraining 512 x 131072 f32 with every rule 105 us, 5.2 TB/s of the 5.4 a copy reaches, by HBM; a choice of 256 x 131072 bf16
+// with every rule 51 us, 3.7 TB/s, by vector issue (41 instructions an entry: nearly every wave has a listed entry at nearly every place, so it is
+// the lists' arithmetic that counts; a loop over what each lane has listed instead took 60 us); a few rows 7 us, by the latency of lists, LDS and logits.
 #include "frl_rows.h"
 
 namespace frl {
@@ -392,7 +395,7 @@ __global__ void __launch_bounds__(G == 64 ? 256 : G, 8) frl_logits_kernel(const 
   }
 }
 
-// the parts of a row joined: one wave per row, a fixed order
+// the parts of a row joined: one wave per row, a fixed order (2 to 5 us, by latency)
 __global__ void __launch_bounds__(256) frl_logits_join_kernel(const LogitsArgs a, long long rows) {
   const int lane = threadIdx.x & 63;
   const long long row = block_index() * 4 + (threadIdx.x >> 6);
