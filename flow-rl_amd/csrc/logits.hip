@@ -46,12 +46,13 @@ __device__ __forceinline__ unsigned long long key_of(float key, unsigned v) {
   return ((unsigned long long)o << 32) | (unsigned)~v;
 }
 
-// x / d with r = 1 / d: the quotient's error is brought back in by one fma (Markstein), which leaves the correctly rounded quotient but
-// where it is subnormal; an infinite quotient stays
-__device__ __forceinline__ float divide(float x, float d, float r) {
-  const float q = x * r;
+// A seen token's logit: x / d where it is positive, else x * d; r = 1 / d.  The quotient's error is brought back in by one fma (Markstein), which
+// leaves the correctly rounded quotient but where it is subnormal; an infinite quotient stays.
+__device__ __forceinline__ float pushed_down(float x, float d, float r) {
+  const bool above = x > 0.0f;
+  const float q = x * (above ? r : d);
   const float q2 = __builtin_fmaf(__builtin_fmaf(-q, d, x), r, q);
-  return q2 == q2 ? q2 : q;
+  return above && q2 == q2 ? q2 : q;
 }
 
 // Entry t of the history: its token (NO_TOKEN for padding), bit 31 set in the prompt
@@ -294,7 +295,7 @@ __global__ void __launch_bounds__(G == 64 ? 256 : G, 8) frl_logits_kernel(const 
         w4 = *(const i32x4*)(w + q * 4 * G + 4 * t0);
         *(i32x4*)(w + q * 4 * G + 4 * t0) = i32x4{0, 0, 0, 0};
       }
-      f32x4 b = {0.0f, 0.0f, 0.0f, 0.0f};
+      f32x4 b = {-0.0f, -0.0f, -0.0f, -0.0f};               // t + -0 is t, whatever t is
       if (a.bias != nullptr && now[q] != 0u) b = load_quad(a.bias + row * a.bias_stride + v, left, 0.0f);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -304,16 +305,15 @@ __global__ void __launch_bounds__(G == 64 ? 256 : G, 8) frl_logits_kernel(const 
           if constexpr (HIST) {
             const unsigned count = SPARSE ? word & COUNT_MASK : word & ~SEEN_IN_PROMPT;
             const unsigned seen = SPARSE ? word & (SEEN_IN_PROMPT | COUNT_MASK) : word;
-            const float pushed = t > 0.0f ? divide(t, rep, rrep) : t * rep;
-            t = seen != 0u ? pushed : t;
+            t = seen != 0u ? pushed_down(t, rep, rrep) : t;
             t = t - (freq * (float)count + (count != 0u ? pres : 0.0f));
           }
-          if (a.bias != nullptr) t = t + b[i];
+          t = t + b[i];
           if constexpr (SPARSE) {
             const unsigned slot = word >> SLOT_SHIFT & SLOT_MASK;
             if (slot != 0u) t = t + val[slot - 1u];
           }
-        } else if (a.bias != nullptr) {
+        } else {
           t = t + b[i];
         }
         const unsigned keep = (unsigned)((int)(now[q] << (31 - i)) >> 31);
