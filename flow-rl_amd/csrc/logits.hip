@@ -11,7 +11,7 @@
 // logits, which are on their way meanwhile.  Two sets of words take turns, so a chunk costs one barrier; a choice keeps its maximum and sum in
 // registers from chunk to chunk and reduces them once.
 // Measured: constraining 512 x 131072 f32 with every rule 105 us, 5.2 TB/s of the 5.4 a copy reaches, by HBM; a choice of 256 x 131072 bf16
-// with every rule 51 us, 3.7 TB/s, by vector issue (41 instructions an entry: nearly every wave has a listed entry at nearly every place, so it is
+// with every rule 50 us, 3.8 TB/s, by vector issue (39 instructions an entry: nearly every wave has a listed entry at nearly every place, so it is
 // the lists' arithmetic that counts; a loop over what each lane has listed instead took 60 us); a few rows 7 us, by the latency of lists, LDS and logits.
 #include "frl_rows.h"
 
