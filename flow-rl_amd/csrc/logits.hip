@@ -424,22 +424,55 @@ __global__ void __launch_bounds__(256) frl_logits_join_kernel(const LogitsArgs a
 
 struct LogitsPlan { int G, chunks, per, parts; };
 
-// Threads per chunk: a wave for short rows; a workgroup of 1024 where lists have to be searched for every chunk and the batch gives every CU two such
-// workgroups; else 256.  A group takes so many chunks of a row that about one round (1024 threads) or two (256) of resident groups remain.  Measured,
-// choice of 256 x 131072 bf16: with a history of 4096, 43 us by 1024 threads in 512 groups, 49 in 1024 groups, 64 by 256 threads; without lists 30 by
-// 1024 threads, 29 by 256.  Constraining 512 x 131072 f32 with a history of 4096: 106 by 1024 threads, 144 by 256; 4096 x 4000 bf16 with a history of
-// 1000: 22 by 256 threads, 37 by 1024; 512 x 131072 f32 with a mask alone: 101 in two rounds, 107 in one.
-static LogitsPlan logits_plan(const FrlLogitsDesc* d) {
-  LogitsPlan p;
-  const long long wide = d->rows * (((long long)d->vocab + 8191) / 8192);
-  const bool lists = d->history_len > 0 || d->n_sparse > 0;
-  p.G = d->vocab <= 512 && d->n_sparse <= 512 ? 64 : (lists && d->vocab > 4096 && wide >= 512) ? 1024 : 256;
-  p.chunks = (int)((d->vocab + 8LL * p.G - 1) / (8 * p.G));
-  const long long rounds = d->rows * p.chunks / (p.G == 1024 ? 512 : 4096);
-  p.per = rounds < 1 ? 1 : rounds > p.chunks ? p.chunks : (int)rounds;
-  p.parts = (p.chunks + p.per - 1) / p.per;
-  p.per = (p.chunks + p.parts - 1) / p.parts;
-  return p;
+// Threads per group and groups per row: a wave for short rows, else what the model below expects to end first.  A group of G threads takes `start` us
+// before its first and after its last chunk (its lists are loaded, its answer is reduced) and `chunk` us a chunk of 8 G entries, both longer
+// by the lists, which every chunk searches (per 1024 entries of them).  The chip holds 2048 groups of 256 threads, which share its issue slots (one on
+// a CU of its own takes ALONE of the time), or 512 of 1024; a choice over several groups of a row pays for the join, its launch and its scratch.
+// The constants are fitted to bf16 calls in which either size was forced, us by 256 / by 1024 threads, with a history of
+//                               64          1024         4096          16384
+//   constrain    1 x  32000    3.8 /  4.5   4.7 /  4.9   7.4 /  5.5   17.8 /  8.4
+//   constrain   64 x 131072   11.1 / 10.0  12.6 / 10.5  18.0 / 11.8   46.1 / 21.2
+//   constrain 4000 x  12000   39   / 49    45   / 55    79   / 63
+//   choose       1 x  32000    7.5 /  9.7   8.4 / 10.3  11.1 / 10.9   22.1 / 13.7
+//   choose     300 x 131072   35   / 43    41   / 46    67   / 51    180   / 92
+//   choose    4000 x   5000   39   / 61    46   / 65    68   / 70
+// Over 25 sizes of each operator with five or six histories the calls it picks are 1.17 times as fast (geometric mean; 0.88 to 3.3 times) as with 1024
+// threads wherever lists meet two such workgroups a CU.  Six candidates for the groups of a row, so that choosing costs well under a microsecond.
+struct GroupCost { float start, start_list, chunk, chunk_list; };
+
+static LogitsPlan logits_plan(const FrlLogitsDesc* d, bool choose) {
+  static const GroupCost COST[2][2] = {              // constrain, choose; 256, 1024 threads
+      {{0.4f, 0.3f, 3.1f, 0.72f}, {1.9f, 0.12f, 2.1f, 0.15f}},
+      {{4.2f, 0.2f, 2.3f, 0.78f}, {4.9f, 0.1f, 2.7f, 0.2f}}};
+  const float JOIN = 4.0f, ALONE = 0.45f;
+  LogitsPlan best;
+  best.G = 64;
+  best.chunks = (int)((d->vocab + 511LL) / 512);
+  best.per = best.parts = 1;
+  if (d->vocab <= 512 && d->n_sparse <= 512) return best;
+  const float lists = ((float)d->history_len + (float)d->n_sparse) * (1.0f / 1024.0f), rows = (float)d->rows;
+  float least = INFINITY;
+  for (int w = 0; w < 2; ++w) {
+    const GroupCost& g = COST[choose][w];
+    const int G = w != 0 ? 1024 : 256, chunks = (int)((d->vocab + 8LL * G - 1) / (8 * G));
+    const float slots = w != 0 ? 512.0f : 2048.0f;
+    int last = 0;
+    for (int rounds = 0; rounds <= 5; ++rounds) {            // one group per row; what fills the chip once to four times; one group per chunk
+      const float fill = slots * (float)rounds / fmaxf(rows, 1.0f);
+      int parts = rounds == 0 ? 1 : rounds == 5 || fill >= (float)chunks ? chunks : fill < 1.0f ? 1 : (int)fill;
+      const int per = (chunks + parts - 1) / parts;
+      parts = (chunks + per - 1) / per;
+      if (parts == last) continue;
+      last = parts;
+      const float full = rows * (float)parts / slots, alone = w != 0 ? 1.0f : ALONE + (1.0f - ALONE) * fminf(full, 1.0f);
+      const float cost = fmaxf(full, 1.0f) * (alone * (g.start + (float)per * g.chunk) + lists * (g.start_list + (float)per * g.chunk_list)) + (choose && parts > 1 ? JOIN : 0.0f);
+      if (cost < least) {
+        least = cost;
+        best.G = G; best.chunks = chunks; best.per = per; best.parts = parts;
+      }
+    }
+  }
+  return best;
 }
 
 template <typename T, typename O, bool CHOOSE>
@@ -475,14 +508,14 @@ static int logits_validate(const FrlLogitsDesc* d, bool choose) {
   if (d->mask < FRL_MASK_NONE || d->mask > FRL_MASK_BYTES) { set_error("logits: mask %d invalid", d->mask); return FRL_EINVAL; }
   if (d->vocab > (1 << 30)) { set_error("logits: vocab %d > 2^30", d->vocab); return FRL_EUNSUPPORTED; }
   if (d->n_sparse > 0 && d->history_len > MAX_HISTORY_WITH_SLOTS) { set_error("logits: history_len %d > %d beside listed biases", d->history_len, MAX_HISTORY_WITH_SLOTS); return FRL_EUNSUPPORTED; }
-  if (d->rows > (1LL << 35) || d->rows * logits_plan(d).chunks > (1LL << 35)) { set_error("logits: %lld rows of %d entries are more than 2^35 chunks in one call", (long long)d->rows, d->vocab); return FRL_EUNSUPPORTED; }
+  if (d->rows > (1LL << 35) || d->rows * logits_plan(d, choose).chunks > (1LL << 35)) { set_error("logits: %lld rows of %d entries are more than 2^35 chunks in one call", (long long)d->rows, d->vocab); return FRL_EUNSUPPORTED; }
   const long long V = d->vocab;
   if (d->rows > 1 && d->logits_stride < V) { set_error("logits: row stride %lld < vocab %lld", (long long)d->logits_stride, V); return FRL_EINVAL; }
   if (d->rows > 1 && !choose && d->out_stride < V) { set_error("logits: out row stride %lld < vocab %lld", (long long)d->out_stride, V); return FRL_EINVAL; }
   return FRL_OK;
 }
 
-static int logits_fill(const FrlLogitsDesc* d, const FrlLogitsBufs* b, LogitsArgs& a, int& G) {
+static int logits_fill(const FrlLogitsDesc* d, const FrlLogitsBufs* b, bool choose, LogitsArgs& a, int& G) {
   if (b == nullptr || b->logits == nullptr) { set_error("logits: bufs.logits is NULL"); return FRL_EINVAL; }
   if (d->history_len > 0 && b->history == nullptr) { set_error("logits: bufs.history is NULL (history_len %d)", d->history_len); return FRL_EINVAL; }
   if (d->n_sparse > 0 && (b->bias_tokens == nullptr || b->bias_values == nullptr)) { set_error("logits: bufs.bias_tokens / bias_values is NULL (n_sparse %d)", d->n_sparse); return FRL_EINVAL; }
@@ -493,7 +526,7 @@ static int logits_fill(const FrlLogitsDesc* d, const FrlLogitsBufs* b, LogitsArg
                  nullptr, nullptr, nullptr, nullptr,
                  d->logits_stride, d->out_stride, d->gumbel_stride, d->history_stride, d->bias_stride, d->sparse_stride, d->mask_stride,
                  d->repetition, d->frequency, d->presence, d->temperature, d->vocab, d->ids64, d->history_len, d->n_sparse, d->mask, 0, 0, 0, 0, 0};
-  const LogitsPlan p = logits_plan(d);
+  const LogitsPlan p = logits_plan(d, choose);
   G = p.G;
   a.chunks = p.chunks; a.per = p.per; a.parts = p.parts;
   a.items = (long long)d->rows * p.parts;
@@ -502,7 +535,7 @@ static int logits_fill(const FrlLogitsDesc* d, const FrlLogitsBufs* b, LogitsArg
 }
 
 static size_t logits_workspace(const FrlLogitsDesc* d) {
-  const int parts = logits_plan(d).parts;
+  const int parts = logits_plan(d, true).parts;
   return parts > 1 ? ((size_t)d->rows * parts * 20 + 511) / 256 * 256 : 256;
 }
 
@@ -519,7 +552,7 @@ int frl_logits_constrain(const FrlLogitsDesc* desc, const FrlLogitsBufs* bufs, v
   if (desc->rows == 0) return FRL_OK;
   LogitsArgs a;
   int G;
-  if ((rc = logits_fill(desc, bufs, a, G)) != FRL_OK) return rc;
+  if ((rc = logits_fill(desc, bufs, false, a, G)) != FRL_OK) return rc;
   if (a.out == nullptr) { set_error("logits: bufs.out is NULL"); return FRL_EINVAL; }
   // in place is the very same rows; any other overlap would be read after it was written
   const size_t in_elt = desc->dtype == FRL_ELT_F32 ? 4 : 2, out_elt = desc->out_dtype == FRL_ELT_F32 ? 4 : 2;
@@ -549,7 +582,7 @@ int frl_logits_choose(const FrlLogitsDesc* desc, const FrlLogitsBufs* bufs, void
   if (desc->rows == 0) return FRL_OK;
   LogitsArgs a;
   int G;
-  if ((rc = logits_fill(desc, bufs, a, G)) != FRL_OK) return rc;
+  if ((rc = logits_fill(desc, bufs, true, a, G)) != FRL_OK) return rc;
   if (a.token == nullptr) { set_error("logits: bufs.token is NULL"); return FRL_EINVAL; }
   if (a.gumbel != nullptr && desc->rows > 1 && desc->gumbel_stride < desc->vocab) { set_error("logits: gumbel row stride %lld < vocab %d", (long long)desc->gumbel_stride, desc->vocab); return FRL_EINVAL; }
   if (a.gumbel == nullptr && a.temperature == nullptr && desc->temperature > 0.0f) { set_error("logits: temperature %g > 0 draws: bufs.gumbel is NULL", desc->temperature); return FRL_EINVAL; }
