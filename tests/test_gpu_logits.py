@@ -83,6 +83,7 @@ CASES = [
     (2, 40, dict(hist=9, sparse=2048), "bool"),                             # lists far longer than the row
     (3, 70001, dict(hist=9000, prompt=True, sparse=600, wide=True), "bool"),   # a history that no group keeps in registers
     (560, 9001, dict(hist=5000, prompt=True), None),
+    (5, 9001, dict(hist=1500, prompt=True, sparse=20, wide=True), "words"),  # beyond what 256 threads keep in registers
     (128, 70001, dict(hist=3000, prompt=True, sparse=50), "words"),         # several chunks to a workgroup of 1024 threads
     (4300, 4001, dict(hist=50, sparse=5), "words"),                         # and to one of 256
 ]
