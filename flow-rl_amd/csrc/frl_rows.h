@@ -18,7 +18,7 @@ typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 // gfx950 takes global vector accesses at any byte alignment (the runtime turns unaligned mode on), so odd vocabularies and
-// odd row strides need no peeling; the copies below become one global_load / global_store each.
+// odd row strides are right without peeling (distill.hip peels for speed); the copies below become one global_load / global_store each.
 template <typename V>
 __device__ __forceinline__ V ldu(const void* p) {
   V v;
