@@ -229,7 +229,7 @@ template <bool REST>
 __device__ __forceinline__ float row_loss(const DistillArgs& a, float m, float s, float r, double sum_p, double cross) {
   if (!REST && sum_p == 0.0) return 0.0f;
   const Shift sh(m, a.scale2);
-  double loss = cross + sum_p * ((sh.fast ? (double)sh.M : (double)m * (double)a.scale2) * LN2 + log((double)s));
+  double loss = cross + sum_p * (((double)m * (double)a.scale2 + (double)sh.residue()) * LN2 + log((double)s));
   if constexpr (REST) {
     const double P = 1.0 - sum_p;
     if (P > 0.0) loss += P * log(P * (double)s / (double)r);

@@ -140,25 +140,32 @@ __device__ __forceinline__ int fresh(int tid) {
   return tid;
 }
 
-// 2^((x - m) c).  With a finite product M = m c this is one fma, whose rounding of M shifts every exponent of the row alike; a maximum near
-// the type's lowest value (a row masked throughout) takes the difference first.
+// 2^(x c - R) about a reference R, m c or what stands for it.  Where |m c| is below LIMIT, R is the rounded product M and an exponential is one
+// fma: M is off by at most 2^-9, every exponent of the sum is shifted alike, and whoever takes the sum's logarithm adds residue() back.  Beyond
+// (masked rows of -1e9 or the type's lowest value, forced tokens, tiny temperatures) the rounding of M would be whole powers of two, or more than
+// an exponential can hold from 2^31 on: there R is m c itself and the difference from m is taken first.
 struct Shift {
+  static constexpr float LIMIT = 65536.0f;
   float m, M, c;
   bool fast;
-  __device__ __forceinline__ Shift(float m_, float c_) : m(m_), M(m_ * c_), c(c_) { fast = fabsf(M) < INFINITY; }
+  __device__ __forceinline__ Shift(float m_, float c_) : m(m_), M(m_ * c_), c(c_) { fast = fabsf(M) < LIMIT; }
+  // R - m c, exact but for the last rounding
+  __device__ __forceinline__ float residue() const { return fabsf(M) < LIMIT ? -__builtin_fmaf(m, c, -M) : 0.0f; }
+  // `fast` may be taken back (so that a wave branches as one): the difference's form has the same reference
   template <int N>
   __device__ __forceinline__ void exps(float* x) const {
     if (fast) {
 #pragma unroll
       for (int i = 0; i < N; ++i) x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], c, -M));
     } else {
+      const float back = residue();
 #pragma unroll
-      for (int i = 0; i < N; ++i) x[i] = __builtin_amdgcn_exp2f((x[i] - m) * c);
+      for (int i = 0; i < N; ++i) x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i] - m, c, -back));
     }
   }
-  // the factor that turns a sum with another, lower shift into one with this: the same rounded products as the exponentials', so they cancel
+  // the factor that turns a sum about another, lower reference into one about this
   __device__ __forceinline__ float from(const Shift& o) const {
-    return __builtin_amdgcn_exp2f(fast && o.fast ? o.M - M : (o.m - m) * c);
+    return __builtin_amdgcn_exp2f(fast && o.fast ? o.M - M : __builtin_fmaf(o.m - m, c, o.residue() - residue()));
   }
 };
 
