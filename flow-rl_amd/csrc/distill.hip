@@ -2,9 +2,10 @@
 //
 // Mathematics (include/flowrl_hip.h).  With c = log2(e) / T, a row needs m = max z, s = sum 2^((z - m) c) and, where the
 // teacher's unnamed mass is a class of its own, r = the same sum without the named entries.  Then q = 2^((z - m) c) / s and
-//     L      = sum p (log p - z / T) + sum p * (m / T + log s)   [+ P (log P - log (r / s))]
+//     L      = sum p (log p + (a - z) / T) + sum p * ((m - a) / T + log s)   [+ P (log P - log (r / s))]
 //     dL/dz  = (q - p) / T        named entries   (FRL_DISTILL_TOP: sum p = 1)
 //     dL/dz  = k q / T            the others, k = 1 (FRL_DISTILL_TOP) or 1 - P s / r (FRL_DISTILL_REST with P > 0)
+// with a the largest named logit, so that rows far from zero (and small T) lose no digits: a - z and m - a are not negative.
 // The gradient is therefore one scaled exponential per element plus a correction of `top` elements.
 //
 // HBM-bound for long rows: the logits once, the gradient once.  For a gradient a row lives in the registers of the threads that share it (16
@@ -155,12 +156,12 @@ struct Running {
 };
 
 // What W lanes make of a row's teacher entries: the tokens (into sid, -1 for padding), p (into sp, 0 for padding) and their logits (into sz),
-// sum p and sum p (log p - z / T).  The three loads of an entry are under way together; what follows works on LDS.  FRL_DISTILL_REST needs
+// sum p, the largest of their logits and sum p (log p + (largest - z) / T).  The three loads of an entry are under way together; what follows works on LDS.  FRL_DISTILL_REST needs
 // 1 - sum p, which float32 exponentials would leave without digits: float64.
 template <typename T, int W, bool REST>
-__device__ __forceinline__ void teacher_part(const DistillArgs& a, long long row, const T* z, int lane, int* sid, float* sp, float* sz, double& sum_p, double& cross) {
+__device__ __forceinline__ void teacher_part(const DistillArgs& a, long long row, const T* z, int lane, int* sid, float* sp, float* sz, double& sum_p, double& cross, float& largest) {
   sum_p = cross = 0.0;
-  float tm = -INFINITY, tot = 0.0f;
+  float tm = -INFINITY, tot = 0.0f, zm = -INFINITY;
   const void* ids = (const char*)a.ids + row * a.ids_stride * (a.ids64 ? 8 : 4);
   for (int k = lane; k < a.top; k += W) {
     const long long id = ld_id(ids, k, a.ids64);
@@ -168,9 +169,13 @@ __device__ __forceinline__ void teacher_part(const DistillArgs& a, long long row
     const bool valid = id >= 0 && id < a.vocab;
     sid[k] = valid ? (int)id : -1;
     sp[k] = t;
-    sz[k] = valid ? Elt<T>::get(z[id]) : 0.0f;
+    const float x = valid ? Elt<T>::get(z[id]) : -INFINITY;
+    sz[k] = x;
+    zm = fmaxf(zm, x);
     if (valid) tm = fmaxf(tm, t);
   }
+  zm = lanes_reduce<MaxOp, W>(zm);
+  largest = zm == -INFINITY ? 0.0f : zm;                     // only -inf is named: any number will do, what has p > 0 makes the loss infinite
   if constexpr (!REST) {
     tm = lanes_reduce<MaxOp, W>(tm);
     const float t0 = tm == -INFINITY ? 0.0f : tm;
@@ -183,7 +188,7 @@ __device__ __forceinline__ void teacher_part(const DistillArgs& a, long long row
     float p = 0.0f;
     if (sid[k] >= 0) {
       const float t = sp[k];
-      const double y = (double)sz[k] * (double)a.scale2 * LN2;   // with the rounded log2(e) / T of the exponentials: one temperature throughout
+      const double y = ((double)largest - (double)sz[k]) * (double)a.scale2 * LN2;   // with the rounded log2(e) / T of the exponentials: one temperature throughout
       float lp;
       if constexpr (REST) {
         const double pd = exp((double)t);
@@ -196,7 +201,7 @@ __device__ __forceinline__ void teacher_part(const DistillArgs& a, long long row
         lp = d - log_tot;
         sum_p += (double)p;
       }
-      if (p != 0.0f) cross += (double)p * ((double)lp - y);
+      if (p != 0.0f) cross += (double)p * ((double)lp + y);
     }
     sp[k] = p;
   }
@@ -226,10 +231,10 @@ __device__ __forceinline__ Factors row_factors(float s, float r, double sum_p) {
 }
 
 template <bool REST>
-__device__ __forceinline__ float row_loss(const DistillArgs& a, float m, float s, float r, double sum_p, double cross) {
+__device__ __forceinline__ float row_loss(const DistillArgs& a, float m, float s, float r, double sum_p, double cross, float largest) {
   if (!REST && sum_p == 0.0) return 0.0f;
   const Shift sh(m, a.scale2);
-  double loss = cross + sum_p * (((double)m * (double)a.scale2 + (double)sh.residue()) * LN2 + log((double)s));
+  double loss = cross + sum_p * ((((double)m - (double)largest) * (double)a.scale2 + (double)sh.residue()) * LN2 + log((double)s));
   if constexpr (REST) {
     const double P = 1.0 - sum_p;
     if (P > 0.0) loss += P * log(P * (double)s / (double)r);
@@ -330,6 +335,7 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, 4) frl_distill_row_kernel(c
   constexpr int WAVES = G < 64 ? 1 : G / 64;
   __shared__ float red0[WAVES], red1[WAVES];
   __shared__ double row_p[GPB], row_x[GPB];
+  __shared__ float row_z[GPB];
   const int tid = threadIdx.x % G, grp = G < 64 ? threadIdx.x / G : G == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
   const int nwords = REST ? (a.vocab + 31) / 32 + 1 : 0;
   unsigned* words = lds + (size_t)grp * (nwords + 3 * a.top);
@@ -366,8 +372,9 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, 4) frl_distill_row_kernel(c
   if constexpr (REST) mark_named<G>(a, row, tid, 0, a.vocab, cut.pad, words);
   if (tid < 64) {
     double sum_p, cross;
-    teacher_part<T, G < 64 ? G : 64, REST>(a, row, z, tid, sid, sp, sz, sum_p, cross);
-    if (tid == 0) { row_p[grp] = sum_p; row_x[grp] = cross; }
+    float largest;
+    teacher_part<T, G < 64 ? G : 64, REST>(a, row, z, tid, sid, sp, sz, sum_p, cross, largest);
+    if (tid == 0) { row_p[grp] = sum_p; row_x[grp] = cross; row_z[grp] = largest; }
   }
   Running<REST> run;
   if (nvec > NV * G) run.template stream<T, G>(zv, NV * G, nvec, a.scale2, words, cut.bit(0), t0, GRAD ? (NV + a.kept) * G : 0, kept);
@@ -426,7 +433,7 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, 4) frl_distill_row_kernel(c
     }
   }
   if (tid == 0) {
-    a.rowloss[row] = w * row_loss<REST>(a, m, s, r, sum_p, row_x[grp]);
+    a.rowloss[row] = w * row_loss<REST>(a, m, s, r, sum_p, row_x[grp], row_z[grp]);
     if (a.stats != nullptr) *(f32x4*)(a.stats + 4 * row) = f32x4{m, k.inv_s, k.k_named, k.k_rest};
   }
 }
@@ -479,7 +486,8 @@ __global__ void __launch_bounds__(1024) frl_distill_join_kernel(const DistillArg
     f32x4 st = {0.0f, 0.0f, 0.0f, 0.0f};
     if (w != 0.0f) {
       double sum_p, cross;
-      teacher_part<T, 64, REST>(a, row, (const T*)a.logits + row * a.logits_stride, lane, sid, sp, sz, sum_p, cross);
+      float largest;
+      teacher_part<T, 64, REST>(a, row, (const T*)a.logits + row * a.logits_stride, lane, sid, sp, sz, sum_p, cross, largest);
       float m = -INFINITY, s = 0.0f, r = 0.0f;
       const float* p = a.part + 3 * row * a.segs;
       for (int i = lane; i < a.segs; i += 64) m = fmaxf(m, p[3 * i]);
@@ -492,7 +500,7 @@ __global__ void __launch_bounds__(1024) frl_distill_join_kernel(const DistillArg
       s = wave_reduce<SumOp>(s);
       r = wave_reduce<SumOp>(r);
       const Factors k = row_factors<REST>(s, r, sum_p);
-      value = w * row_loss<REST>(a, m, s, r, sum_p, cross);
+      value = w * row_loss<REST>(a, m, s, r, sum_p, cross, largest);
       st = f32x4{m, k.inv_s, k.k_named, k.k_rest};
     }
     if (lane == 0) {
@@ -551,7 +559,8 @@ __global__ void __launch_bounds__(G == 64 ? 256 : G) frl_distill_grad_kernel(con
   if (lone >= 0) g[v0 + lone] = Elt<T>::put(sc.one(Elt<T>::get(z[v0 + lone])));
   if (tid < 64) {
     double sum_p, cross;
-    teacher_part<T, 64, REST>(a, row, z, tid, sid, sp, sz, sum_p, cross);
+    float largest;
+    teacher_part<T, 64, REST>(a, row, z, tid, sid, sp, sz, sum_p, cross, largest);
   }
   group_sync<G>();
   named_gradient<T, G>(a, g, v0, n, sh, f * st[2] * st[1], f, sid, sp, sz, tid);

@@ -69,3 +69,50 @@ def test_gradient_over_the_temperatures(N, V, K, T, kind):
         _, g, _, tolg = rows_of(z[pick], ids[pick], t[pick], kind, T)
         losses, grads = _grads(z, ids, t, T, kind)
         _check_gradients(grads, pick, g, tolg)
+
+
+def _check_losses(losses, pick, L, tolL):
+    for got in losses:
+        a = got[pick].double().cpu().numpy()
+        assert (np.abs(a - L) <= tolL + 2.0 ** -24 * np.abs(L)).all(), f"{a} vs {L}, bounds {tolL}"
+
+
+@pytest.mark.parametrize("fill", [-1e5, -1e9, -1e20, -3.4e38, 1e5, 1e10, 1e30])
+@pytest.mark.parametrize("N,V,K", SHAPES)
+def test_loss_of_students_far_from_zero(N, V, K, fill):
+    """The divergence depends on differences of logits only: the same for a row of 1e30 as for a row of 0."""
+    import torch
+    rng = np.random.default_rng(V + 2)
+    for dtype in (torch.float32, torch.bfloat16):
+        z, ids, t = make_distill(rng, N, V, K, "logits", dtype)
+        level = torch.tensor(max(fill, torch.finfo(dtype).min)).to(dtype)
+        z[0] = level
+        z[1] = level
+        z[1, ids[1]] = 2 * level if fill > 0 else level / 2      # named entries ahead of the others by more than an exponential spans
+        pick = _picked(N)
+        L, _, tolL, _ = rows_of(z[pick], ids[pick], t[pick], "logits", 1.0)
+        losses, _ = _grads(z, ids, t, 1.0, "logits")
+        _check_losses(losses, pick, L, tolL)
+        # the rest as a class, of a row that its rules leave uniform
+        u = torch.log_softmax(torch.from_numpy(t).double(), 1).add(np.log(0.7)).float().numpy()
+        L, _, tolL, _ = rows_of(z[:1], ids[:1], u[:1], "logprobs", 1.0)
+        losses, _ = _grads(z, ids, u, 1.0, "logprobs")
+        _check_losses(losses, [0], L, tolL)
+
+
+@pytest.mark.parametrize("T", [1e-30, 1e-9, 1e-6, 1e-3, 1e6, 1e30])
+@pytest.mark.parametrize("N,V,K", SHAPES)
+def test_loss_over_the_temperatures(N, V, K, T):
+    """A teacher whose best entry is the student's: at small temperatures both are certain of it, and the divergence is what their doubts differ by."""
+    import torch
+    rng = np.random.default_rng(V + 3)
+    T = float(np.float32(T))
+    for dtype in (torch.float32, torch.bfloat16):
+        z, ids, t = make_distill(rng, N, V, K, "logits", dtype)
+        best, mine = z.float().argmax(1).numpy(), t.argmax(1)
+        keep = ~(ids == best[:, None]).any(1)
+        ids[keep, mine[keep]] = best[keep]
+        pick = _picked(N)
+        L, _, tolL, _ = rows_of(z[pick], ids[pick], t[pick], "logits", T)
+        losses, _ = _grads(z, ids, t, T, "logits")
+        _check_losses(losses, pick, L, tolL)
