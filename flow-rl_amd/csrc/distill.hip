@@ -1,10 +1,13 @@
 // KL divergence of a student's softmax from a teacher's top entries, and its gradient: frl_distill_fwd / frl_distill_bwd.
 //
-// Mathematics (include/flowrl_hip.h).  With c = log2(e) / T, a row needs m = max z, s = sum 2^((z - m) c) and, where the
-// teacher's unnamed mass is a class of its own, r = the same sum without the named entries.  Then q = 2^((z - m) c) / s and
-//     L      = sum p (log p + (a - z) / T) + sum p * ((m - a) / T + log s)   [+ P (log P - log (r / s))]
-//     dL/dz  = (q - p) / T        named entries   (FRL_DISTILL_TOP: sum p = 1)
-//     dL/dz  = k q / T            the others, k = 1 (FRL_DISTILL_TOP) or 1 - P s / r (FRL_DISTILL_REST with P > 0)
+// Mathematics (include/flowrl_hip.h).  With c = log2(e) / T, a row needs m = max z and s = sum 2^((z - m) c); where the teacher's unnamed mass is a
+// class of its own, its entries ("the rest") have a maximum m' and a sum r = sum 2^((z - m') c) of theirs, and the named entries another pair: the
+// rest of a student that is sure of what is named, or of a vocabulary masked beside it, lies further below m than an exponential spans, and
+// still has a divergence and a gradient.  Then q = 2^((z - m) c) / s, Q = 2^((m' - m) c) r / s and
+//     L      = sum p (log p + (a - z) / T) + sum p * ((m - a) / T + log s)   [+ P (log P - log Q)]
+//     dL/dz  = (q - p) / T                              named entries   (FRL_DISTILL_TOP: sum p = 1)
+//     dL/dz  = q / T, or                                the others, FRL_DISTILL_TOP
+//              2^((z - m') c) (Q - P) / (r T)           the others, FRL_DISTILL_REST with P > 0
 // with a the largest named logit, so that rows far from zero (and small T) lose no digits: a - z and m - a are not negative.
 // The gradient is therefore one scaled exponential per element plus a correction of `top` elements.
 //
@@ -22,11 +25,12 @@ namespace frl {
 struct DistillArgs {
   const void* logits; const void* ids; const void* teacher; const float* weights;
   float* rowloss;             // (rows,) weight * L
-  float* stats;               // (rows + 1, 4) or NULL: m, 1 / s, factor of the named entries, factor of the others; last row: 1 / denominator
+  float* stats;               // (rows + 1, 4) or NULL: m, factor of 2^((z - m) c) of the named entries, m', factor of 2^((z - m') c) of the others; last
+                              // row: 1 / denominator
   const float* inv_denom;     // device 1 / sum of weights, or NULL: `denom_scale`
   const float* g_loss;        // backward: cotangent, `g_stride` apart per row (0: one scalar); NULL: 1
   void* grad;
-  float* part;                // split rows: (rows, segs, 3) m, s, r
+  float* part;                // split rows: (rows, segs, 4) maximum and sum of the rest (FRL_DISTILL_TOP: of everything), of the named entries
   long long rows, logits_stride, grad_stride, ids_stride, teacher_stride;
   float inv_temp, scale2, denom_scale;   // 1 / T, log2(e) / T
   int vocab, top, ids64, teacher_dtype, segs, seg_len, g_stride;
@@ -84,24 +88,53 @@ __device__ __forceinline__ float sum_of(const float* e) {
 template <int N>
 __device__ __forceinline__ unsigned named_bits(const unsigned* words, int v) { return (words[v >> 5] >> (v & 31)) & ((1u << N) - 1u); }
 
-template <int N>
-__device__ __forceinline__ float sum_unnamed(const float* e, unsigned named) {
-  float s = 0.0f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) s += (named >> i & 1u) ? 0.0f : e[i];
-  return s;
-}
-
-// A thread's share of a row that is streamed: its own running maximum, and sums that it rescales when a batch raises the maximum.
-template <bool REST>
+// A thread's running maximum, and a sum that it rescales when something raises the maximum.
 struct Running {
-  float m = -INFINITY, s = 0.0f, r = 0.0f;
+  float m = -INFINITY, s = 0.0f;
   __device__ __forceinline__ void raise(float to, float c) {
     if (to > m) {
       about(to, c);
       m = to;
     }
   }
+  __device__ __forceinline__ void one(float x, float c) {
+    raise(x, c);
+    Shift(m == -INFINITY ? 0.0f : m, c).exps<1>(&x);
+    s += x;
+  }
+  // the sum with respect to a maximum over more threads; a thread that saw only -inf has a sum of 0 (or NaN) and keeps it
+  __device__ __forceinline__ void about(float all, float c) {
+    if (m != -INFINITY) s *= Shift(all, c).from(Shift(m, c));
+  }
+};
+
+// Named entries among a vector's N: they go into a sum of their own, and -inf takes their place among the rest.  Few vectors have one.
+template <typename T>
+__device__ __forceinline__ void take_named(u32x4& raw, unsigned named, float c, Running& of_named) {
+  const unsigned ninf = Vec16<T>::fill_minus_inf()[0];
+  while (named != 0u) {
+    const int i = __builtin_ctz(named), w = sizeof(T) == 4 ? i : i >> 1;
+    named &= named - 1u;
+    const unsigned word = w == 0 ? raw[0] : w == 1 ? raw[1] : w == 2 ? raw[2] : raw[3];
+    unsigned mask = 0xffffffffu;
+    float x;
+    if constexpr (sizeof(T) == 4) {
+      x = __uint_as_float(word);
+    } else {
+      mask = (i & 1) ? 0xffff0000u : 0x0000ffffu;
+      x = Elt<T>::get(T{(unsigned short)((i & 1) ? word >> 16 : word)});
+    }
+    const unsigned without = (word & ~mask) | (ninf & mask);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) raw[j] = j == w ? without : raw[j];
+    of_named.one(x, c);
+  }
+}
+
+// A thread's share of a row that is streamed
+template <bool REST>
+struct Share {
+  Running run, of_named;                                   // without REST everything is in `run`
   // vectors [from, to) of the vectors at z, G threads apart; the first one's named bits begin at bit0.  Those before `keep` stay in LDS (at `kept`) for
   // the same thread's gradient.
   template <typename T, int G>
@@ -116,42 +149,48 @@ struct Running {
         for (int u = 0; u < U; ++u)
           if (at + u * G < keep) kept[at + u * G - from] = raw[u];
       }
-      float bm = m;
+      if constexpr (REST) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (at + u * G < to) take_named<T>(raw[u], named_bits<N>(words, bit0 + (at + u * G) * N), c, of_named);
+      }
+      float bm = run.m;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         float x[N];
         Vec16<T>::unpack(raw[u], x);
         bm = max_of<N>(x, bm);
       }
-      raise(bm, c);
-      const Shift sh(m == -INFINITY ? 0.0f : m, c);
+      run.raise(bm, c);
+      const Shift sh(run.m == -INFINITY ? 0.0f : run.m, c);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         float x[N];
         Vec16<T>::unpack(raw[u], x);
         sh.exps<N>(x);
-        const float e = sum_of<N>(x);
-        s += e;
-        if constexpr (REST) {
-          const unsigned named = at + u * G < to ? named_bits<N>(words, bit0 + (at + u * G) * N) : 0u;
-          r += named == 0u ? e : sum_unnamed<N>(x, named);
-        }
+        run.s += sum_of<N>(x);
       }
     }
   }
   __device__ __forceinline__ void one(float x, float c, bool named) {
-    raise(x, c);
-    Shift(m == -INFINITY ? 0.0f : m, c).template exps<1>(&x);
-    s += x;
-    if (REST && !named) r += x;
+    if constexpr (REST) of_named.one(named ? x : -INFINITY, c);      // of -inf there is nothing to add; a branch would put both sums into memory
+    run.one(named ? -INFINITY : x, c);
   }
-  // the sums with respect to a maximum over more threads; a thread that saw only -inf has sums of 0 (or NaN) and keeps them
-  __device__ __forceinline__ void about(float all, float c) {
-    if (m != -INFINITY) {
-      const float f = Shift(all, c).from(Shift(m, c));
-      s *= f;
-      r *= f;
+};
+
+// A row's maximum and sum, and the rest's (FRL_DISTILL_TOP: the same)
+struct Sums {
+  float m, s, mr, r, down;                                 // down: the rest's sum times this is about the row's reference
+  template <bool REST>
+  static __device__ __forceinline__ Sums of(float mr, float r, float mn, float n, float c) {
+    Sums o = {mr, r, mr, r, 1.0f};
+    if constexpr (REST) {
+      o.m = fmaxf(mr, mn);
+      const Shift sh(o.m, c);
+      o.down = mr == -INFINITY ? 0.0f : sh.from(Shift(mr, c));
+      o.s = (mr == -INFINITY ? r : r * o.down) + (mn == -INFINITY ? n : n * sh.from(Shift(mn, c)));      // of -inf alone a sum is 0 (or NaN)
     }
+    return o;
   }
 };
 
@@ -211,33 +250,35 @@ __device__ __forceinline__ void teacher_part(const DistillArgs& a, long long row
 
 __device__ __forceinline__ float inverse(double s) { return s != 0.0 ? (float)(1.0 / s) : 0.0f; }
 
-struct Factors { float inv_s, k_named, k_rest; };
+// The gradient is T^-1 times the cotangent times: named 2^((z - m) c) - p, and rest 2^((z - m') c)
+struct Factors { float named, rest; };
 
 template <bool REST>
-__device__ __forceinline__ Factors row_factors(float s, float r, double sum_p) {
-  Factors o;
-  o.inv_s = 1.0f / s;
-  o.k_named = o.k_rest = (float)sum_p;
+__device__ __forceinline__ Factors row_factors(const Sums& t, double sum_p) {
+  const float inv_s = 1.0f / t.s;
   if constexpr (REST) {
     const double P = 1.0 - sum_p;
-    if (P > 0.0) {
-      o.k_named = 1.0f;
-      o.k_rest = 1.0f - (float)P * s / r;
-    }
-  } else if (sum_p == sum_p) {
-    o.k_named = o.k_rest = sum_p != 0.0 ? 1.0f : 0.0f;     // a softmax sums to one; a row that names nothing has neither loss nor gradient
+    if (P > 0.0) return Factors{inv_s, t.r == 0.0f ? 0.0f : t.down * inv_s - (float)P / t.r};      // an empty rest has no gradient
+    return Factors{(float)sum_p * inv_s, (float)sum_p * t.down * inv_s};
+  } else {
+    // a softmax sums to one; a row that names nothing has neither loss nor gradient
+    const float k = sum_p != sum_p ? (float)sum_p * inv_s : sum_p != 0.0 ? inv_s : 0.0f;
+    return Factors{k, k};
   }
-  return o;
 }
 
 template <bool REST>
-__device__ __forceinline__ float row_loss(const DistillArgs& a, float m, float s, float r, double sum_p, double cross, float largest) {
+__device__ __forceinline__ float row_loss(const DistillArgs& a, const Sums& t, double sum_p, double cross, float largest) {
   if (!REST && sum_p == 0.0) return 0.0f;
-  const Shift sh(m, a.scale2);
-  double loss = cross + sum_p * ((((double)m - (double)largest) * (double)a.scale2 + (double)sh.residue()) * LN2 + log((double)s));
+  const double c = (double)a.scale2, m = (double)t.m;
+  const double log_s = (double)Shift(t.m, a.scale2).residue() * LN2 + log((double)t.s);
+  double loss = cross + sum_p * ((m - (double)largest) * c * LN2 + log_s);
   if constexpr (REST) {
     const double P = 1.0 - sum_p;
-    if (P > 0.0) loss += P * log(P * (double)s / (double)r);
+    if (P > 0.0) {
+      const double log_r = (double)Shift(t.mr, a.scale2).residue() * LN2 + log((double)t.r);
+      loss += P * (log(P) + (m - (double)t.mr) * c * LN2 + log_s - log_r);
+    }
   }
   return (float)loss;
 }
@@ -376,48 +417,51 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, 4) frl_distill_row_kernel(c
     teacher_part<T, G < 64 ? G : 64, REST>(a, row, z, tid, sid, sp, sz, sum_p, cross, largest);
     if (tid == 0) { row_p[grp] = sum_p; row_x[grp] = cross; row_z[grp] = largest; }
   }
-  Running<REST> run;
-  if (nvec > NV * G) run.template stream<T, G>(zv, NV * G, nvec, a.scale2, words, cut.bit(0), t0, GRAD ? (NV + a.kept) * G : 0, kept);
-  if (lone >= 0) run.one(Elt<T>::get(z[lone]), a.scale2, REST && named_bits<1>(words, lone + cut.pad) != 0u);
-  float m = run.m;
+  Share<REST> mine;
+  if (nvec > NV * G) mine.template stream<T, G>(zv, NV * G, nvec, a.scale2, words, cut.bit(0), t0, GRAD ? (NV + a.kept) * G : 0, kept);
+  if (lone >= 0) mine.one(Elt<T>::get(z[lone]), a.scale2, REST && named_bits<1>(words, lone + cut.pad) != 0u);
+  float mr = mine.run.m;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
     if (i < nv) {
+      if constexpr (REST)
+        if (i * G + t0 < nvec) take_named<T>(raw[i], named_bits<N>(words, cut.bit(i * G + t0)), a.scale2, mine.of_named);
       float x[N];
       Vec16<T>::unpack(raw[i], x);
-      m = max_of<N>(x, m);
+      mr = max_of<N>(x, mr);
       __builtin_amdgcn_sched_barrier(0);
     }
-  m = group_reduce<MaxOp, G>(m, red0);
-  run.about(m, a.scale2);
-  const Shift sh(m, a.scale2);
+  mr = group_reduce<MaxOp, G>(mr, red0);
+  const float mn = REST ? group_reduce<MaxOp, G>(mine.of_named.m, red1) : -INFINITY;
+  mine.run.about(mr, a.scale2);
+  const Shift sh(mr == -INFINITY ? 0.0f : mr, a.scale2);
   keep_packed<NV>(raw);
-  const int t1 = fresh(tid);
 #pragma unroll
   for (int i = 0; i < NV; ++i)
     if (i < nv) {
       float x[N];
       Vec16<T>::unpack(raw[i], x);
       sh.exps<N>(x);
-      const float e = sum_of<N>(x);
-      run.s += e;
-      if constexpr (REST) {
-        const unsigned named = i * G + t1 < nvec ? named_bits<N>(words, cut.bit(i * G + t1)) : 0u;
-        run.r += named == 0u ? e : sum_unnamed<N>(x, named);
-      }
+      mine.run.s += sum_of<N>(x);
       __builtin_amdgcn_sched_barrier(0);                     // one vector unpacked at a time: eight independent elements are parallel enough
     }
-  const float s = group_reduce<SumOp, G>(run.s, red1);
-  const float r = REST ? group_reduce<SumOp, G>(run.r, red0) : 0.0f;   // red0: every thread has read the maximum before the barrier in the sum
+  // two arrays in turn: between a result that is read and the next that is written into the same one lies the other's barrier
+  const float r = group_reduce<SumOp, G>(mine.run.s, REST ? red0 : red1);
+  float n = 0.0f;
+  if constexpr (REST) {
+    mine.of_named.about(mn, a.scale2);
+    n = group_reduce<SumOp, G>(mine.of_named.s, red1);
+  }
   if constexpr (G <= 64) group_sync<G>();                    // the teacher's part is visible (a workgroup has passed barriers since)
+  const Sums sums = Sums::of<REST>(mr, r, mn, n, a.scale2);
   const double sum_p = row_p[grp];
-  const Factors k = row_factors<REST>(s, r, sum_p);
+  const Factors k = row_factors<REST>(sums, sum_p);
   if constexpr (GRAD) {
     const float f = w * inv * a.inv_temp;
-    if (k.k_named == 0.0f && k.k_rest == 0.0f) {
+    if (k.named == 0.0f && k.rest == 0.0f) {
       zero_row<T, G>(g, a.vocab, tid);
     } else {
-      const Scaled<T> sc(sh, f * k.k_rest * k.inv_s);
+      const Scaled<T> sc(sh, f * k.rest);
       keep_packed<NV>(raw);
       const int t2 = fresh(tid);
 #pragma unroll
@@ -429,12 +473,12 @@ __global__ void __launch_bounds__(G <= 64 ? 256 : G, 4) frl_distill_row_kernel(c
       if (nvec > NV * G) stream_gradient<T, G>(zv, g + cut.head, NV * G, nvec, sc, t2, (NV + a.kept) * G, kept);
       if (lone >= 0) g[lone] = Elt<T>::put(sc.one(Elt<T>::get(z[lone])));
       group_sync<G>();
-      named_gradient<T, G>(a, g, 0, a.vocab, sh, f * k.k_named * k.inv_s, f, sid, sp, sz, tid);
+      named_gradient<T, G>(a, g, 0, a.vocab, Shift(sums.m, a.scale2), f * k.named, f, sid, sp, sz, tid);
     }
   }
   if (tid == 0) {
-    a.rowloss[row] = w * row_loss<REST>(a, m, s, r, sum_p, row_x[grp], row_z[grp]);
-    if (a.stats != nullptr) *(f32x4*)(a.stats + 4 * row) = f32x4{m, k.inv_s, k.k_named, k.k_rest};
+    a.rowloss[row] = w * row_loss<REST>(a, sums, sum_p, row_x[grp], row_z[grp]);
+    if (a.stats != nullptr) *(f32x4*)(a.stats + 4 * row) = f32x4{sums.m, k.named, sums.mr, k.rest};
   }
 }
 
@@ -458,16 +502,18 @@ __global__ void __launch_bounds__(G) frl_distill_part_kernel(const DistillArgs a
   const Cut<T> cut(z, n);
   const int lone = cut.lone(tid);
   if constexpr (REST) mark_named<G>(a, row, tid, v0, n, cut.pad, lds);
-  Running<REST> run;
-  run.template stream<T, G>(z + cut.head, 0, cut.nvec, a.scale2, lds, cut.bit(0), tid);
-  if (lone >= 0) run.one(Elt<T>::get(z[lone]), a.scale2, REST && named_bits<1>(lds, lone + cut.pad) != 0u);
-  const float m = group_reduce<MaxOp, G>(run.m, red0);
-  run.about(m, a.scale2);
-  const float s = group_reduce<SumOp, G>(run.s, red1), r = REST ? group_reduce<SumOp, G>(run.r, red0) : 0.0f;   // red0: read before the barrier in the sum
-  if (threadIdx.x == 0) {
-    float* p = a.part + 3 * item;
-    p[0] = m; p[1] = s; p[2] = r;
+  Share<REST> mine;
+  mine.template stream<T, G>(z + cut.head, 0, cut.nvec, a.scale2, lds, cut.bit(0), tid);
+  if (lone >= 0) mine.one(Elt<T>::get(z[lone]), a.scale2, REST && named_bits<1>(lds, lone + cut.pad) != 0u);
+  const float mr = group_reduce<MaxOp, G>(mine.run.m, red0), mn = REST ? group_reduce<MaxOp, G>(mine.of_named.m, red1) : -INFINITY;
+  mine.run.about(mr, a.scale2);
+  const float r = group_reduce<SumOp, G>(mine.run.s, REST ? red0 : red1);                 // the arrays in turn, as in the row kernel
+  float named = 0.0f;
+  if constexpr (REST) {
+    mine.of_named.about(mn, a.scale2);
+    named = group_reduce<SumOp, G>(mine.of_named.s, red1);
   }
+  if (threadIdx.x == 0) *(f32x4*)(a.part + 4 * item) = f32x4{mr, r, mn, named};
 }
 
 // One wave per row: the segments joined in order, then the teacher's entries.  A workgroup of 16 waves that holds every row finishes the loss as well.
@@ -488,20 +534,25 @@ __global__ void __launch_bounds__(1024) frl_distill_join_kernel(const DistillArg
       double sum_p, cross;
       float largest;
       teacher_part<T, 64, REST>(a, row, (const T*)a.logits + row * a.logits_stride, lane, sid, sp, sz, sum_p, cross, largest);
-      float m = -INFINITY, s = 0.0f, r = 0.0f;
-      const float* p = a.part + 3 * row * a.segs;
-      for (int i = lane; i < a.segs; i += 64) m = fmaxf(m, p[3 * i]);
-      m = wave_reduce<MaxOp>(m);
+      float mr = -INFINITY, mn = -INFINITY, r = 0.0f, n = 0.0f;
+      const float* p = a.part + 4 * row * a.segs;
       for (int i = lane; i < a.segs; i += 64) {
-        const float f = p[3 * i] == -INFINITY ? 1.0f : Shift(m, a.scale2).from(Shift(p[3 * i], a.scale2));     // a segment of -inf alone has sums of 0 (or NaN)
-        s += p[3 * i + 1] * f;
-        r += p[3 * i + 2] * f;
+        mr = fmaxf(mr, p[4 * i]);
+        mn = fmaxf(mn, p[4 * i + 2]);
       }
-      s = wave_reduce<SumOp>(s);
+      mr = wave_reduce<MaxOp>(mr);
+      mn = wave_reduce<MaxOp>(mn);
+      for (int i = lane; i < a.segs; i += 64) {              // a segment of -inf alone has a sum of 0 (or NaN)
+        const f32x4 v = *(const f32x4*)(p + 4 * i);
+        r += v[0] == -INFINITY ? v[1] : v[1] * Shift(mr, a.scale2).from(Shift(v[0], a.scale2));
+        n += v[2] == -INFINITY ? v[3] : v[3] * Shift(mn, a.scale2).from(Shift(v[2], a.scale2));
+      }
       r = wave_reduce<SumOp>(r);
-      const Factors k = row_factors<REST>(s, r, sum_p);
-      value = w * row_loss<REST>(a, m, s, r, sum_p, cross, largest);
-      st = f32x4{m, k.inv_s, k.k_named, k.k_rest};
+      n = wave_reduce<SumOp>(n);
+      const Sums sums = Sums::of<REST>(mr, r, mn, n, a.scale2);
+      const Factors k = row_factors<REST>(sums, sum_p);
+      value = w * row_loss<REST>(a, sums, sum_p, cross, largest);
+      st = f32x4{sums.m, k.named, sums.mr, k.rest};
     }
     if (lane == 0) {
       a.rowloss[row] = value;
@@ -545,14 +596,13 @@ __global__ void __launch_bounds__(G == 64 ? 256 : G) frl_distill_grad_kernel(con
   T* g = (T*)a.grad + row * a.grad_stride;
   const float w = a.weights != nullptr ? a.weights[row] : 1.0f;
   const f32x4 st = *(const f32x4*)(a.stats + 4 * row);
-  if (w == 0.0f || (st[2] == 0.0f && st[3] == 0.0f)) {
+  if (w == 0.0f || (st[1] == 0.0f && st[3] == 0.0f)) {
     zero_row<T, G>(g + v0, n, tid);
     return;
   }
   const float cot = a.g_loss != nullptr ? a.g_loss[row * a.g_stride] : 1.0f;
   const float f = cot * w * inv * a.inv_temp;
-  const Shift sh(st[0], a.scale2);
-  const Scaled<T> sc(sh, f * st[3] * st[1]);
+  const Scaled<T> sc(Shift(st[2] == -INFINITY ? 0.0f : st[2], a.scale2), f * st[3]);
   const Cut<T> cut(z + v0, n);
   const int lone = cut.lone(tid);
   stream_gradient<T, G>(z + v0 + cut.head, g + v0 + cut.head, 0, cut.nvec, sc, tid);
@@ -563,7 +613,7 @@ __global__ void __launch_bounds__(G == 64 ? 256 : G) frl_distill_grad_kernel(con
     teacher_part<T, 64, REST>(a, row, z, tid, sid, sp, sz, sum_p, cross, largest);
   }
   group_sync<G>();
-  named_gradient<T, G>(a, g, v0, n, sh, f * st[2] * st[1], f, sid, sp, sz, tid);
+  named_gradient<T, G>(a, g, v0, n, Shift(st[0], a.scale2), f * st[1], f, sid, sp, sz, tid);
 }
 
 // ---- over the rows ------------------------------------------------------------------------------------------------------
@@ -689,7 +739,7 @@ static DistillWs distill_ws(const FrlDistillDesc* d, const DistillPlan& p) {
   w.inv = up((size_t)d->rows);
   w.stats = w.inv + 64;
   w.part = w.stats + up(4 * (size_t)(d->rows + 1));
-  w.total = (w.part + (p.split ? up(3 * (size_t)d->rows * p.segs) : 0)) * sizeof(float);
+  w.total = (w.part + (p.split ? up(4 * (size_t)d->rows * p.segs) : 0)) * sizeof(float);
   return w;
 }
 

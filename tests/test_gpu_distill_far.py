@@ -55,7 +55,7 @@ def test_gradient_of_students_far_from_zero(N, V, K, fill, kind):
         _check_gradients(grads, pick, g, tolg)
 
 
-@pytest.mark.parametrize("kind", ["logits"])
+@pytest.mark.parametrize("kind", ["logits", "logprobs"])
 @pytest.mark.parametrize("T", [1e-30, 1e-9, 1e-6, 1e-3, 1e6, 1e30])
 @pytest.mark.parametrize("N,V,K", SHAPES)
 def test_gradient_over_the_temperatures(N, V, K, T, kind):
@@ -116,3 +116,51 @@ def test_loss_over_the_temperatures(N, V, K, T):
         L, _, tolL, _ = rows_of(z[pick], ids[pick], t[pick], "logits", T)
         losses, _ = _grads(z, ids, t, T, "logits")
         _check_losses(losses, pick, L, tolL)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("gap", [60.0, 100.0, 1e4])
+@pytest.mark.parametrize("N,V,K", SHAPES)
+def test_a_rest_far_below(N, V, K, gap, dtype):
+    """The teacher's unnamed mass is a class of its own, of which a student that is sure of the named entries keeps e^-gap: its divergence is near
+    P gap and the rest's gradient is minus the rest's own distribution times P, with numbers throughout."""
+    import torch
+    rng = np.random.default_rng(V + 4)
+    z, ids, t = make_distill(rng, N, V, K, "logprobs", getattr(torch, dtype), ragged=True)
+    r = np.arange(N)
+    z[0, ids[0, 0]] += gap                               # one named entry is ahead
+    named = np.zeros((N, V), bool)
+    for k in range(K):
+        ok = (ids[:, k] >= 0) & (ids[:, k] < V)
+        named[r[ok], ids[ok, k]] = True
+    z[1:][torch.from_numpy(named[1:])] += gap            # all of them are
+    z[2][torch.from_numpy(~named[2])] = -gap             # the rest is one masked level
+    z[N - 1][torch.from_numpy(~named[N - 1] & (rng.random(V) < 0.5))] = float("-inf")
+    if N > 3:
+        t[N // 2] += 1.0 - np.log(np.exp(t[N // 2].astype(np.float64)).sum())       # names more than all there is: no rest
+    for T in (1.0, 0.5):
+        pick = _picked(N)
+        L, g, tolL, tolg = rows_of(z[pick], ids[pick], t[pick], "logprobs", T)
+        assert np.isfinite(L).all()
+        losses, grads = _grads(z, ids, t, T, "logprobs")
+        _check_losses(losses, pick, L, tolL)
+        _check_gradients(grads, pick, g, tolg)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("N,V,K", SHAPES)
+def test_a_rest_of_nothing(N, V, K, dtype):
+    """Mass that is left where the student has none, neither below nor beside what is named: an infinite divergence, gradients that are numbers, 0 at
+    the entries that are ruled out."""
+    import torch
+    rng = np.random.default_rng(V + 5)
+    z, ids, t = make_distill(rng, N, V, K, "logprobs", getattr(torch, dtype))
+    named = torch.zeros((N, V), dtype=torch.bool).scatter_(1, torch.from_numpy(ids).long(), True)
+    z[1][~named[1]] = float("-inf")
+    pick = _picked(N)
+    L, g, tolL, tolg = rows_of(z[pick], ids[pick], t[pick], "logprobs", 1.0)
+    losses, grads = _grads(z, ids, t, 1.0, "logprobs")
+    for got in losses:
+        assert float(got[1]) == float("inf") and torch.isfinite(got[torch.arange(N, device="cuda") != 1]).all()
+    _check_gradients(grads, pick, g, tolg)
+    assert not any(got[1].cpu()[~named[1]].any() for got in grads)
