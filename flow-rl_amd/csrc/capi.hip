@@ -798,8 +798,8 @@ size_t frl_critic_workspace_bytes(const FrlCriticDesc* desc) {
   return critic_ws_floats(desc, pl, hoist) * sizeof(float);
 }
 
-int frl_critic_select(const FrlCriticDesc* desc, const FrlCriticParams* params, const FrlSelectBufs* bufs,
-                      void* workspace, size_t workspace_bytes, void* hip_stream) {
+static int critic_select(const FrlCriticDesc* desc, const FrlCriticParams* params, const FrlSelectBufs* bufs, const CandidateMask& mask,
+                         void* workspace, size_t workspace_bytes, void* hip_stream) {
   clear_kernels();
   FrlDesc d; Plan pl; bool hoist;
   int rc = critic_plan(desc, d, pl, hoist);
@@ -854,7 +854,21 @@ int frl_critic_select(const FrlCriticDesc* desc, const FrlCriticParams* params, 
     if (rc != FRL_OK) return rc;
   }
   return launch_critic_select(qm, E, desc->n_states, desc->particles, pl.A, bufs->actions, bufs->gumbel, bufs->inv_temperature,
-                              bufs->q, bufs->best_idx, bufs->best_action, stream);
+                              mask, bufs->q, bufs->best_idx, bufs->best_action, stream);
+}
+
+int frl_critic_select(const FrlCriticDesc* desc, const FrlCriticParams* params, const FrlSelectBufs* bufs,
+                      void* workspace, size_t workspace_bytes, void* hip_stream) {
+  return critic_select(desc, params, bufs, CandidateMask{nullptr, 0, FRL_MASK_NONE}, workspace, workspace_bytes, hip_stream);
+}
+
+int frl_critic_select_masked(const FrlCriticDesc* desc, const FrlCriticParams* params, const FrlSelectBufs* bufs,
+                             const void* allowed, int32_t mask, int64_t mask_stride,
+                             void* workspace, size_t workspace_bytes, void* hip_stream) {
+  if (mask < FRL_MASK_NONE || mask > FRL_MASK_BYTES) { set_error("critic select: mask %d invalid", mask); return FRL_EINVAL; }
+  if ((mask != FRL_MASK_NONE) != (allowed != nullptr)) { set_error("critic select: allowed must be non-NULL exactly when mask is set"); return FRL_EINVAL; }
+  if (mask_stride < 0) { set_error("critic select: mask_stride %lld < 0", (long long)mask_stride); return FRL_EINVAL; }
+  return critic_select(desc, params, bufs, CandidateMask{allowed, mask_stride, mask}, workspace, workspace_bytes, hip_stream);
 }
 
 // ---- sampler + critic scoring + selection in one launch ----------------------------------------------------------------

@@ -3,15 +3,18 @@
 //   flowrl/agent/offline/dql.py:155-161   qs.min(axis=0).reshape(B, N); argmax / categorical; actions[arange(B), idx]
 //   flowrl/agent/online/qvpo.py:40-43     same with argmax
 // HBM-bound and tiny next to the scoring MLP: 4 (E + 1) bytes per candidate read, A + 1 words per state written.
-// One wave per state; lanes stride over the candidates, ties resolve to the LOWEST index (jnp.argmax).
+// One wave per state; lanes stride over the candidates, ties resolve to the LOWEST index and a NaN is above everything (jnp.argmax).  A mask rules
+// candidates out before their keys are looked at; what is chosen among the others does not depend on it.
 #include "frl_internal.h"
 
 namespace frl {
 
+__device__ __forceinline__ bool ahead(float a, float b) { return a > b || (a != a && b == b); }
+
 __global__ void __launch_bounds__(256) frl_critic_select_kernel(const float* __restrict__ qm, int E, long long n_states, int N, int A,
                                                                 const float* __restrict__ actions, const float* __restrict__ gumbel,
-                                                                float inv_temp, float* __restrict__ q, int32_t* __restrict__ best_idx,
-                                                                float* __restrict__ best_action) {
+                                                                float inv_temp, const CandidateMask mask, float* __restrict__ q,
+                                                                int32_t* __restrict__ best_idx, float* __restrict__ best_action) {
   const int lane = threadIdx.x & 63;
   const long long B = n_states * N;
   for (long long s = (long long)blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6); s < n_states;
@@ -23,20 +26,23 @@ __global__ void __launch_bounds__(256) frl_critic_select_kernel(const float* __r
       float v = qm[c];
       for (int e = 1; e < E; ++e) v = fminf(v, qm[(size_t)e * B + c]);     // qs.min(axis=0)
       if (q != nullptr) q[c] = v;
+      if (mask.kind == FRL_MASK_WORDS && !(((const unsigned*)mask.allowed)[s * mask.stride + (p >> 5)] >> (p & 31) & 1u)) continue;
+      if (mask.kind == FRL_MASK_BYTES && ((const unsigned char*)mask.allowed)[s * mask.stride + p] == 0) continue;
       const float key = (gumbel != nullptr) ? fmaf(v, inv_temp, gumbel[c]) : v; // categorical == argmax(logits + Gumbel)
-      if (bi == 0x7fffffff || key > best) { best = key; bi = p; }           // strict >: the first maximum wins
+      if (bi == 0x7fffffff || ahead(key, best)) { best = key; bi = p; }     // strictly: the first maximum wins
     }
     // wave reduction: larger key wins, equal keys -> smaller index
     for (int off = 32; off >= 1; off >>= 1) {
       const float ob = __shfl_xor(best, off);
       const int oi = __shfl_xor(bi, off);
-      const bool take = (oi != 0x7fffffff) && (bi == 0x7fffffff || ob > best || (ob == best && oi < bi));
+      const bool take = (oi != 0x7fffffff) && (bi == 0x7fffffff || ahead(ob, best) || (!ahead(best, ob) && oi < bi));
       if (take) { best = ob; bi = oi; }
     }
-    if (best_idx != nullptr && lane == 0) best_idx[s] = bi;
+    const bool none = bi == 0x7fffffff;                   // every candidate is ruled out
+    if (best_idx != nullptr && lane == 0) best_idx[s] = none ? -1 : bi;
     if (best_action != nullptr) {
-      const float* src = actions + (s * N + bi) * (long long)A;
-      for (int a = lane; a < A; a += 64) best_action[s * A + a] = src[a];
+      const float* src = actions + (s * N + (none ? 0 : bi)) * (long long)A;
+      for (int a = lane; a < A; a += 64) best_action[s * A + a] = none ? __builtin_nanf("") : src[a];
     }
   }
 }
@@ -55,13 +61,13 @@ int launch_critic_tab(const CriticPtrs& v, const float** dst, hipStream_t stream
 }
 
 int launch_critic_select(const float* q_members, int E, long long n_states, int particles, int A, const float* actions,
-                         const float* gumbel, float inv_temperature, float* q, int32_t* best_idx, float* best_action,
-                         hipStream_t stream) {
+                         const float* gumbel, float inv_temperature, const CandidateMask& mask, float* q, int32_t* best_idx,
+                         float* best_action, hipStream_t stream) {
   if (n_states <= 0) return FRL_OK;
   const long long blocks = (n_states + 3) / 4;
   const int grid = (int)(blocks < 4096 ? blocks : 4096);
   hipLaunchKernelGGL(frl_critic_select_kernel, dim3(grid), dim3(256), 0, stream, q_members, E, n_states, particles, A, actions,
-                     gumbel, inv_temperature, q, best_idx, best_action);
+                     gumbel, inv_temperature, mask, q, best_idx, best_action);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) { set_error("critic select launch: %s", hipGetErrorString(e)); return FRL_EHIP; }
   return FRL_OK;

@@ -504,9 +504,10 @@ int launch_cond_embed(int act, const float* obs, long long n_states, int in_dim,
 int launch_state_bias(const float* obs, long long n_states, int in_dim, int H, const float* w, const float* b, float* zs,
                       hipStream_t stream);
 int launch_critic_tab(const CriticPtrs& v, const float** dst, hipStream_t stream);
+struct CandidateMask { const void* allowed; long long stride; int kind; };      // which candidates may be chosen: FRL_MASK_*
 int launch_critic_select(const float* q_members, int E, long long n_states, int particles, int A, const float* actions,
-                         const float* gumbel, float inv_temperature, float* q, int32_t* best_idx, float* best_action,
-                         hipStream_t stream);
+                         const float* gumbel, float inv_temperature, const CandidateMask& mask, float* q, int32_t* best_idx,
+                         float* best_action, hipStream_t stream);
 int launch_random_uniform(const uint32_t* key, int impl, long long n, float lo, float hi, float* out, hipStream_t stream);
 int launch_random_randint(const uint32_t* key, int impl, long long n, int32_t minval, int32_t maxval, int32_t* out, hipStream_t stream);
 // csrc/net_eval.hip: per-sample-time evaluation rows and the forward-process pieces

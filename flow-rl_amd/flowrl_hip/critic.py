@@ -111,7 +111,8 @@ def critic_select(critic: Ensemblize, params: Dict, obs: Optional[torch.Tensor],
     qs (B, N) = min over the ensemble).  temperature <= 0: argmax (dql.py:156-157); temperature > 0: the categorical
     draw of dql.py:158-160 as argmax(qs / (1e-6 + T) + gumbel) with ``gumbel`` (B, N) supplied by the caller.
     ``allowed`` (no counterpart in the reference): which candidates may be chosen, as :class:`flowrl_hip.logits.Constraints` takes it
-    (bool (B, N), or int32 words); a state whose candidates are all ruled out answers idx -1 and an action of NaN."""
+    (bool (B, N), or int32 words, or one row for every state); what they leave is chosen from as without it, on the same noise; a state whose
+    candidates are all ruled out answers idx -1 and an action of NaN."""
     lib = _lib.load()
     if not actions.is_cuda:
         raise RuntimeError("flowrl_hip critic scoring runs on the GPU only; there is no CPU fallback")
@@ -121,16 +122,7 @@ def critic_select(critic: Ensemblize, params: Dict, obs: Optional[torch.Tensor],
     B = actions.numel() // (A * N)
     if B * N * A != actions.numel():
         raise ValueError("actions do not hold num_samples candidates per state")
-    if allowed is not None:
-        drawn = temperature is not None and temperature > 0.0
-        if drawn and gumbel is None:
-            raise ValueError("temperature > 0 draws from a categorical: pass gumbel=(B, N) Gumbel(0,1) noise")
-        _, _, q = critic_select(critic, params, obs, actions, N)
-        idx, _ = logits.choose(q, logits.Constraints(allowed=allowed), temperature=float(temperature) if drawn else 0.0,
-                               gumbel=gumbel.reshape(B, N) if drawn else None)
-        some = (idx >= 0)[:, None]
-        best = torch.where(some, actions.reshape(B, N, A).gather(1, idx.long().clamp(min=0)[:, None, None].expand(B, 1, A))[:, 0], torch.nan)
-        return best, idx, (q if want_q else None)
+    mask, which, stride = (None, _lib.FRL_MASK_NONE, 0) if allowed is None else logits._allowed(allowed, B, N, dev.index)
     d, fp, bufs, keep, (best, idx, q) = _critic_marshal(critic, params, obs, B, N, A, dev, temperature, gumbel, want_q)
     act2 = _f32c(actions.reshape(B * N, A), dev, "actions")
     bufs.actions = act2.data_ptr()
@@ -140,8 +132,8 @@ def critic_select(critic: Ensemblize, params: Dict, obs: Optional[torch.Tensor],
         raise _lib.FlowRLHipUnsupported(_lib.FRL_EUNSUPPORTED, "this critic configuration has no kernel")
     ws = _workspace(need, dev, torch.cuda.current_stream(dev).cuda_stream)
     with torch.cuda.device(dev):
-        rc = lib.frl_critic_select(C.byref(d), C.byref(fp), C.byref(bufs), ws.data_ptr(), ws.numel(),
-                                   torch.cuda.current_stream(dev).cuda_stream)
+        rc = lib.frl_critic_select_masked(C.byref(d), C.byref(fp), C.byref(bufs), None if mask is None else mask.data_ptr(), which, stride,
+                                          ws.data_ptr(), ws.numel(), torch.cuda.current_stream(dev).cuda_stream)
     _lib.check(rc)
     return best, idx, q
 

@@ -139,6 +139,18 @@ def _ids(t: torch.Tensor, what: str) -> int:
     return wide
 
 
+def _allowed(t: torch.Tensor, R: int, V: int, index: int) -> Tuple[torch.Tensor, int, int]:
+    """(tensor, FRL_MASK_*, row stride) of a mask over V entries"""
+    if t.dtype is torch.bool:
+        mask, n = _lib.FRL_MASK_BYTES, V
+    elif t.dtype is torch.int32:
+        mask, n = _lib.FRL_MASK_WORDS, (V + 31) // 32
+    else:
+        raise TypeError(f"allowed: bool entries or int32 words of 32 entries required (got {t.dtype})")
+    t, stride = _rows_of(t, R, n, index, "allowed", True)
+    return t, mask, stride
+
+
 def _no_grad(what: str, *ts) -> None:
     for t in ts:
         if isinstance(t, torch.Tensor) and t.requires_grad:
@@ -209,13 +221,7 @@ def _marshal(z: torch.Tensor, R: int, V: int, c: Constraints, z_stride: Optional
         raise ValueError("bias_values without bias_tokens")
     allowed = c.allowed
     if allowed is not None:
-        if allowed.dtype is torch.bool:
-            mask, n = _lib.FRL_MASK_BYTES, V
-        elif allowed.dtype is torch.int32:
-            mask, n = _lib.FRL_MASK_WORDS, (V + 31) // 32
-        else:
-            raise TypeError(f"allowed: bool entries or int32 words of 32 entries required (got {allowed.dtype})")
-        allowed, m_stride = _rows_of(allowed, R, n, index, "allowed", True)
+        allowed, mask, m_stride = _allowed(allowed, R, V, index)
         a_ptr = allowed.data_ptr()
     d, b = _lib.FrlLogitsDesc(), _lib.FrlLogitsBufs()
     _DESC.pack_into(d, 0, _lib.FRL_ABI_VERSION, _ELT[z.dtype], out_elt, V, R, ids64, L, K, mask, V if z_stride is None else z_stride, out_stride, gumbel_stride,

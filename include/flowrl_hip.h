@@ -313,6 +313,11 @@ typedef struct FrlCriticParams {
   const float* bias[FRL_MAX_HIDDEN + 1];   /* backbone/Dense_i/bias (E, H); [L] = the head bias (E, 1) */
 } FrlCriticParams;
 
+/* What an `allowed` operand holds */
+#define FRL_MASK_NONE 0
+#define FRL_MASK_WORDS 1 /* int32 words: bit v & 31 of word v >> 5 set = entry v is allowed */
+#define FRL_MASK_BYTES 2 /* one byte per entry, non-zero = allowed (a bool tensor) */
+
 typedef struct FrlSelectBufs {
   const float* obs;      /* (n_states, S), NULL iff obs_dim == 0 */
   const float* actions;  /* (n_states * particles, A): the sampler's x0 */
@@ -328,6 +333,14 @@ size_t frl_critic_workspace_bytes(const FrlCriticDesc* desc);
 /* E launches of the fused MFMA network kernel (one evaluation per chain, no update rule) + one selection kernel. */
 int frl_critic_select(const FrlCriticDesc* desc, const FrlCriticParams* params, const FrlSelectBufs* bufs,
                       void* workspace, size_t workspace_bytes, void* hip_stream);
+
+/* The same choice among the candidates that `allowed` leaves (no counterpart in the reference): `mask` FRL_MASK_WORDS,
+ * ceil(particles / 32) int32 words a state, or FRL_MASK_BYTES, `particles` bytes a state, FRL_MASK_NONE with allowed = NULL;
+ * states are mask_stride words / bytes apart, 0: one row of them for every state.  Every candidate is scored (q); a state
+ * whose candidates are all ruled out has best_idx -1 and a best_action of NaN. */
+int frl_critic_select_masked(const FrlCriticDesc* desc, const FrlCriticParams* params, const FrlSelectBufs* bufs,
+                             const void* allowed, int32_t mask, int64_t mask_stride,
+                             void* workspace, size_t workspace_bytes, void* hip_stream);
 
 /* Sampler + critic scoring + selection in ONE launch (SURVEY 8(f) rank 1 as written: jit_sample_and_select dql.py:130-162,
  * jit_sample_actions qvpo.py:21-44).  frl_sampler_fwd followed by frl_critic_select, except that the candidate actions
@@ -478,10 +491,6 @@ int frl_mse_loss(int64_t n, const float* pred, const float* target, float* loss,
 #define FRL_ELT_BF16 1
 #define FRL_ELT_F16 2
 
-#define FRL_MASK_NONE 0
-#define FRL_MASK_WORDS 1 /* int32 words: bit v & 31 of word v >> 5 set = allowed */
-#define FRL_MASK_BYTES 2 /* one byte per entry, non-zero = allowed (a bool tensor) */
-
 #define FRL_LOGITS_MAX_SPARSE 2048 /* entries of one row's bias_tokens list; more than that is a dense bias */
 
 typedef struct FrlLogitsDesc {
@@ -522,7 +531,8 @@ typedef struct FrlLogitsBufs {
 int frl_logits_constrain(const FrlLogitsDesc* desc, const FrlLogitsBufs* bufs, void* hip_stream);
 
 /* One entry per row of the constrained logits, without writing them.  With T = temperature > 0 and noise: y = x * (1 /
- * (1e-6 + T)) (the factor at least FLT_MIN) and token = argmax(y + gumbel), the categorical draw of frl_critic_select; else y = x and token = argmax(y).
+ * (1e-6 + T)) (the factor at least FLT_MIN) and token = argmax(y + gumbel), a categorical draw (frl_critic_select's key rounds once; this one's product
+ * and sum are rounded each, so that with the same noise the two may part where keys lie within a rounding); else y = x and token = argmax(y).
  * The first of equal maxima; a NaN counts as the largest value (argmax's rule in jax and torch).  logprob = y[token] -
  * log sum exp y.  A row that its rules leave nothing (every y is -inf) answers token -1, logprob -inf.
  * frl_logits_workspace_bytes: 0 for a bad descriptor; 256 where a call needs no scratch and takes workspace = NULL. */
