@@ -161,8 +161,9 @@ def distill_loss(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor,
                  weights: Optional[torch.Tensor] = None, reduction: str = "mean") -> torch.Tensor:
     """:func:`flowrl_hip.logits.distill_loss` as a differentiable torch op: the backward is one pass over the logits from the row statistics the
     forward kept (frl_distill_bwd).  Gradients flow to ``logits``; the teacher and the weights are not differentiated and asking
-    for it raises.  Forward and backward can be captured into a graph together, as any torch backward can: while no eager graph of the
+    for it raises, as forward-mode tangents do.  Forward and backward can be captured into a graph together, as any torch backward can: while no eager graph of the
     same leaves is alive."""
+    _logits._no_tangent("logits / teacher / weights", logits, teacher, weights)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (teacher, weights)):
         raise NotImplementedError("flowrl_hip.autograd: distill_loss differentiates the student's logits only; detach teacher / weights")
     if not (torch.is_grad_enabled() and logits.requires_grad):

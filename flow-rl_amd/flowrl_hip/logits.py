@@ -25,6 +25,7 @@ from dataclasses import dataclass
 from typing import Optional, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _lib
 
@@ -151,7 +152,20 @@ def _allowed(t: torch.Tensor, R: int, V: int, index: int) -> Tuple[torch.Tensor,
     return t, mask, stride
 
 
+def _no_tangent(what: str, *ts) -> None:
+    """Refuse operands that carry a forward-mode tangent (no_grad leaves those alone): it would be dropped."""
+    if getattr(_forward_ad, "_current_level", 0) < 0:      # outside of every dual_level
+        return
+    for t in ts:
+        if isinstance(t, torch.Tensor) and _forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"flowrl_hip.logits: {what} has a forward-mode tangent, which is not carried on; unpack_dual it")
+
+
 def _no_grad(what: str, *ts) -> None:
+    """Refuse operands whose derivative would be lost."""
+    _no_tangent(what, *ts)
+    if not torch.is_grad_enabled():
+        return
     for t in ts:
         if isinstance(t, torch.Tensor) and t.requires_grad:
             raise NotImplementedError(f"flowrl_hip.logits: {what} is not differentiated here; detach it")
@@ -247,8 +261,7 @@ def constrain(logits: torch.Tensor, rules: Optional[Constraints] = None, *, out:
     """The logits with ``rules`` applied, in the logits' type or float32 (``out_dtype``), rounded once.  ``out``: where they go, a
     tensor of the logits' shape with contiguous rows; it may be ``logits`` itself."""
     rules = _NO_RULES if rules is None else rules
-    if torch.is_grad_enabled():
-        _no_grad("logits / a rule / out", logits, out, *_differentiable(rules))
+    _no_grad("logits / a rule / out", logits, out, *_differentiable(rules))
     z, R, V, stride = _check_logits(logits, "logits")
     index = logits.get_device()
     given = out is not None
@@ -286,8 +299,7 @@ def choose(logits: torch.Tensor, rules: Optional[Constraints] = None, *, tempera
     first of equal maxima; NaN counts as the largest.  logprob is log softmax of y (of the constrained logits for a greedy row).  A row
     that the rules leave nothing answers token -1 with logprob -inf."""
     rules = _NO_RULES if rules is None else rules
-    if torch.is_grad_enabled():
-        _no_grad("logits / a rule / the temperature", logits, temperature, *_differentiable(rules))
+    _no_grad("logits / a rule / the temperature", logits, temperature, *_differentiable(rules))      # nothing that has a derivative depends on the noise
     z, R, V, stride = _check_logits(logits, "logits")
     index = logits.get_device()
     t = g = None
@@ -378,7 +390,6 @@ def distill_loss(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor,
     ``weights`` (rows,) float32: a row of weight 0 is not read.  ``reduction`` "mean" divides by the sum of the weights; "none" returns
     the rows' weighted divergences.  With ``want_grad`` also d loss / d logits in the logits' type, in the same pass ("none": of
     the rows' sum).  Like ``mse_loss`` a value without a graph; :func:`flowrl_hip.autograd.distill_loss` differentiates."""
-    if torch.is_grad_enabled():
-        _no_grad("logits (use flowrl_hip.autograd.distill_loss) / teacher / weights", logits, teacher, weights)
+    _no_grad("logits (use flowrl_hip.autograd.distill_loss) / teacher / weights", logits, teacher, weights)
     loss, grad, _ = distill_forward(logits, ids, teacher, kind, temperature, weights, reduction, want_grad)
     return (loss, grad) if want_grad else loss

@@ -2,7 +2,10 @@
 import ctypes as C
 
 import pytest
+import torch
+import torch.autograd.forward_ad as fad
 
+import flowrl_hip as fh
 from flowrl_hip import _lib
 
 
@@ -23,3 +26,27 @@ def test_masked_selection_refuses(lib, allowed, mask, stride):
     assert b"mask" in lib.frl_last_error()
     # and what the entry point without a mask refuses
     assert lib.frl_critic_select_masked(C.byref(d), C.byref(p), C.byref(b), None, _lib.FRL_MASK_NONE, 0, None, 0, None) == _lib.FRL_EWORKSPACE
+
+
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("where", ["logits", "rule", "out", "temperature", "teacher", "weights", "leaf"])
+def test_forward_mode_tangents_are_refused(where, grad):
+    """A dual operand needs no requires_grad, and no_grad leaves its tangent alone: it must not be dropped in silence."""
+    z, ids, t, w = torch.zeros((2, 8)), torch.zeros((2, 1), dtype=torch.int32), torch.zeros((2, 1)), torch.ones(2)
+    with fad.dual_level(), torch.set_grad_enabled(grad):
+        dual = lambda x: fad.make_dual(x, torch.ones_like(x))  # noqa: E731
+        calls = {
+            "logits": [lambda: fh.logits.constrain(dual(z)), lambda: fh.logits.choose(dual(z)), lambda: fh.logits.distill_loss(dual(z), ids, t),
+                       lambda: fh.autograd.distill_loss(dual(z), ids, t)],
+            "rule": [lambda: fh.logits.constrain(z, fh.logits.Constraints(bias=dual(z[0]))), lambda: fh.logits.choose(z, fh.logits.Constraints(presence=dual(w)))],
+            "out": [lambda: fh.logits.constrain(z, out=dual(z.clone()))],
+            "temperature": [lambda: fh.logits.choose(z, temperature=dual(w))],
+            "teacher": [lambda: fh.logits.distill_loss(z, ids, dual(t)), lambda: fh.autograd.distill_loss(z, ids, dual(t))],
+            "weights": [lambda: fh.logits.distill_loss(z, ids, t, weights=dual(w)), lambda: fh.autograd.distill_loss(z, ids, t, weights=dual(w))],
+            "leaf": [lambda: fh.autograd.distill_loss(dual(z.clone().requires_grad_(True)), ids, t)],
+        }[where]
+        for call in calls:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        with pytest.raises(RuntimeError, match="GPU only"):
+            fh.logits.choose(z)
