@@ -712,10 +712,8 @@ static int distill_validate(const FrlDistillDesc* d) {
 }
 
 static bool distill_overlap(const FrlDistillDesc* d, const FrlDistillBufs* b) {
-  const size_t elt = d->dtype == FRL_ELT_F32 ? 4 : 2;
-  const uintptr_t i0 = (uintptr_t)b->logits, i1 = i0 + ((size_t)(d->rows - 1) * d->logits_stride + d->vocab) * elt;
-  const uintptr_t o0 = (uintptr_t)b->grad, o1 = o0 + ((size_t)(d->rows - 1) * d->grad_stride + d->vocab) * elt;
-  return i0 < o1 && o0 < i1;
+  const long long elt = d->dtype == FRL_ELT_F32 ? 4 : 2, width = d->vocab * elt;
+  return rows_overlap((uintptr_t)b->logits, width, d->logits_stride * elt, (uintptr_t)b->grad, width, d->grad_stride * elt, d->rows);
 }
 
 static DistillArgs distill_args(const FrlDistillDesc* d, const FrlDistillBufs* b, const DistillPlan& p) {

@@ -183,6 +183,16 @@ inline dim3 grid_of(long long blocks) {
 }
 __device__ __forceinline__ long long block_index() { return (long long)blockIdx.y * gridDim.x + blockIdx.x; }
 
+// Whether rows of wa bytes, sa bytes apart from a on, share a byte with rows of wb bytes, sb apart from b on (a distance is no less than its rows).  Rows
+// at one distance may lie between one another, as the column blocks of one buffer do; of different distances only ranges that do not meet are
+// taken to be apart.
+inline bool rows_overlap(uintptr_t a, long long wa, long long sa, uintptr_t b, long long wb, long long sb, long long rows) {
+  if (a >= b + (uintptr_t)((rows - 1) * sb + wb) || b >= a + (uintptr_t)((rows - 1) * sa + wa)) return false;
+  if (rows == 1 || sa != sb) return true;
+  const long long apart = (long long)(b - a) % sa, d = apart < 0 ? apart + sa : apart;      // where a row of b begins behind the last row of a
+  return d < wa || d + wb > sa;
+}
+
 struct MaxOp {
   static __device__ __forceinline__ float f(float a, float b) { return fmaxf(a, b); }
   static __device__ __forceinline__ unsigned long long f(unsigned long long a, unsigned long long b) { return a > b ? a : b; }

@@ -555,11 +555,9 @@ int frl_logits_constrain(const FrlLogitsDesc* desc, const FrlLogitsBufs* bufs, v
   if ((rc = logits_fill(desc, bufs, false, a, G)) != FRL_OK) return rc;
   if (a.out == nullptr) { set_error("logits: bufs.out is NULL"); return FRL_EINVAL; }
   // in place is the very same rows; any other overlap would be read after it was written
-  const size_t in_elt = desc->dtype == FRL_ELT_F32 ? 4 : 2, out_elt = desc->out_dtype == FRL_ELT_F32 ? 4 : 2;
-  const uintptr_t i0 = (uintptr_t)a.logits, i1 = i0 + ((size_t)(desc->rows - 1) * desc->logits_stride + desc->vocab) * in_elt;
-  const uintptr_t o0 = (uintptr_t)a.out, o1 = o0 + ((size_t)(desc->rows - 1) * desc->out_stride + desc->vocab) * out_elt;
-  const bool same = i0 == o0 && desc->dtype == desc->out_dtype && (desc->logits_stride == desc->out_stride || desc->rows == 1);
-  if (!same && i0 < o1 && o0 < i1) { set_error("logits: out overlaps logits without being the same rows"); return FRL_EINVAL; }
+  const long long in_elt = desc->dtype == FRL_ELT_F32 ? 4 : 2, out_elt = desc->out_dtype == FRL_ELT_F32 ? 4 : 2, V = desc->vocab;
+  const bool same = a.logits == a.out && desc->dtype == desc->out_dtype && (desc->logits_stride == desc->out_stride || desc->rows == 1);
+  if (!same && rows_overlap((uintptr_t)a.logits, V * in_elt, desc->logits_stride * in_elt, (uintptr_t)a.out, V * out_elt, desc->out_stride * out_elt, desc->rows)) { set_error("logits: out overlaps logits without being the same rows"); return FRL_EINVAL; }
   const bool f32 = desc->out_dtype == FRL_ELT_F32;
   hipStream_t st = (hipStream_t)hip_stream;
   hipError_t e = hipErrorInvalidValue;

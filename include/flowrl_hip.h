@@ -510,7 +510,8 @@ typedef struct FrlLogitsDesc {
 
 typedef struct FrlLogitsBufs {
   const void* logits;             /* (rows, vocab) */
-  void* out;                      /* (rows, vocab); constrain only.  May be `logits` itself (same type and stride) */
+  void* out;                      /* (rows, vocab); constrain only.  May be `logits` itself (same type and stride); else no entry in common
+                                   * (rows may lie between the logits' rows where both are as many bytes apart) */
   const void* history;            /* (rows, history_len) tokens */
   const int32_t* lengths;         /* (rows,) or NULL: every row is full */
   const int32_t* prompt_lengths;  /* (rows,) or NULL: no prompt */
@@ -580,7 +581,8 @@ typedef struct FrlDistillBufs {
   float* row_stats;     /* (rows + 1, FRL_DISTILL_STATS): fwd writes it (NULL: not wanted), bwd reads it */
   const float* g_loss;  /* bwd: dL/d loss, scalar or (rows,) */
   void* grad;           /* (rows, vocab), dtype: bwd's result; fwd with grad != NULL also writes d loss / d logits in the same
-                           call (FRL_REDUCE_NONE: of the rows' sum).  Must not overlap logits */
+                           call (FRL_REDUCE_NONE: of the rows' sum).  No entry in common with logits (rows may lie between theirs
+                           where both are as many apart) */
 } FrlDistillBufs;
 
 size_t frl_distill_workspace_bytes(const FrlDistillDesc* desc);

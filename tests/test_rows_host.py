@@ -50,3 +50,34 @@ def test_forward_mode_tangents_are_refused(where, grad):
                 call()
         with pytest.raises(RuntimeError, match="GPU only"):
             fh.logits.choose(z)
+
+
+V = 1000
+
+
+def _rows(**kw):
+    d = _lib.FrlLogitsDesc()
+    d.abi_version, d.dtype, d.out_dtype, d.vocab, d.rows, d.repetition = _lib.FRL_ABI_VERSION, _lib.FRL_ELT_BF16, _lib.FRL_ELT_BF16, V, 7, 1.0
+    d.logits_stride = d.out_stride = 2 * V
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+# entries from the first logit to the first result; two bytes each
+@pytest.mark.parametrize("off,kw", [(V - 1, {}), (1, {}), (V + 1, {}), (2 * V - 1, {}), (-1, {}), (-(V - 1), {}), (-(V + 1), {}), (2 * V, {}), (-2 * V, {}), (12 * V, {}),
+                                    (13 * V - 1, {}), (-12 * V, {}), (-(13 * V - 1), {}), (V, dict(out_stride=2 * V + 1)), (V, dict(out_dtype=_lib.FRL_ELT_F32, out_stride=V)),
+                                    (V, dict(out_dtype=_lib.FRL_ELT_F32, out_stride=2 * V)), (V - 1, dict(rows=1)), (0, dict(out_stride=2 * V + 2))])
+def test_results_that_share_entries_with_logits_are_refused(lib, off, kw):
+    d, b = _rows(**kw), _lib.FrlLogitsBufs()
+    b.logits, b.out = 1 << 30, (1 << 30) + 2 * off
+    assert lib.frl_logits_constrain(C.byref(d), C.byref(b), None) == _lib.FRL_EINVAL
+    assert b"overlaps" in lib.frl_last_error()
+    if not kw:
+        d = _lib.FrlDistillDesc()
+        d.abi_version, d.dtype, d.vocab, d.top, d.rows, d.temperature = _lib.FRL_ABI_VERSION, _lib.FRL_ELT_BF16, V, 4, 7, 1.0
+        d.logits_stride = d.grad_stride = 2 * V
+        b = _lib.FrlDistillBufs()
+        b.logits, b.ids, b.teacher, b.loss, b.grad, b.row_stats, b.g_loss = 1 << 30, 1 << 12, 1 << 13, 1 << 14, (1 << 30) + 2 * off, 1 << 16, 1 << 15
+        for rc in (lib.frl_distill_fwd(C.byref(d), C.byref(b), 4096, 1 << 30, None), lib.frl_distill_bwd(C.byref(d), C.byref(b), None)):
+            assert rc == _lib.FRL_EINVAL and b"overlaps" in lib.frl_last_error()
