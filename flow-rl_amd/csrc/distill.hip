@@ -801,7 +801,7 @@ static hipError_t launch_grad(const DistillArgs& a, const DistillPlan& p, hipStr
   if (wave) hipLaunchKernelGGL((frl_distill_grad_kernel<T, 64, REST>), grid, dim3(256), lds, st, a);
   else if (p.G == 256) hipLaunchKernelGGL((frl_distill_grad_kernel<T, 256, REST>), grid, dim3(256), lds, st, a);
   else hipLaunchKernelGGL((frl_distill_grad_kernel<T, 1024, REST>), grid, dim3(1024), lds, st, a);
-  note_kernel("frl_distill_grad_kernel<%d threads> [%lld]", p.G, blocks);
+  note_kernel("frl_distill_grad_kernel<%d threads> [%lld]", wave ? 64 : p.G == 256 ? 256 : 1024, blocks);
   return hipGetLastError();
 }
 

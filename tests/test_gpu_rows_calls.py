@@ -46,3 +46,23 @@ def test_results_between_the_logits_rows(R, V, gap):
             assert torch.equal(src, z) and (buf[:, rest] == 5.0).all()
             assert abs(float(out - loss)) <= 2.0 ** -16 * R * 10
             assert float((dst.float() - grad.float()).abs().max()) <= (2.0 ** -16 if dtype == torch.float32 else 2.0 ** -8)
+
+
+def _built():
+    from flowrl_hip import _lib
+    return _lib.load().frl_last_kernels().decode()
+
+
+@pytest.mark.parametrize("N,V,value,grad", [(70000, 100, 16, 64), (70000, 300, 64, 64), (600, 5001, 512, 1024), (2048, 3001, 256, 256), (300, 70001, 1024, 1024), (3, 50001, 256, 256)])
+def test_the_builds_that_are_named_are_those_that_ran(N, V, value, grad):
+    """frl_last_kernels after the forward and after the backward."""
+    import torch
+    import flowrl_hip as fh
+    z = torch.zeros((N, V), dtype=torch.bfloat16, device="cuda")
+    ids, t = torch.zeros((N, 1), dtype=torch.int32, device="cuda"), torch.zeros((N, 1), device="cuda")
+    loss, _, stats = fh.logits.distill_forward(z, ids, t, "logits", 1.0, None, "sum", want_stats=True)
+    forward = _built()
+    fh.logits.distill_backward(z, ids, t, "logits", 1.0, None, "sum", stats, torch.ones((), device="cuda"))
+    backward = _built()
+    assert f"<value, {value} threads" in forward or (N < 256 and "frl_distill_part_kernel" in forward), forward
+    assert f"frl_distill_grad_kernel<{grad} threads>" in backward, backward
