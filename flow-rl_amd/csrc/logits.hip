@@ -86,7 +86,8 @@ __device__ __forceinline__ void stage_listed(const LogitsArgs& a, long long row,
     for (int k = tid; k < a.K; k += G) {
       if (tok[k] == NO_TOKEN) continue;
       const unsigned mine = tok[k] + 1u;
-      for (unsigned i = mine * 2654435761u, probe = 0; probe < SLOTS; ++probe, ++i) {
+      // the product's highest bits: its lowest would be the token's own, the same for tokens a multiple of SLOTS apart
+      for (unsigned i = mine * 2654435761u >> (32 - __builtin_ctz(SLOTS)), probe = 0; probe < SLOTS; ++probe, ++i) {
         const unsigned was = atomicCAS(&table[i % SLOTS], 0u, mine);
         if (was == mine) *several = 1;
         if (was == 0u || was == mine) break;
