@@ -47,7 +47,7 @@ __device__ __forceinline__ unsigned long long key_of(float key, unsigned v) {
 }
 
 // A seen token's logit: x / d where it is positive, else x * d; r = 1 / d.  The quotient's error is brought back in by one fma (Markstein), which
-// leaves the correctly rounded quotient but where it is subnormal; an infinite quotient stays.
+// leaves the correctly rounded quotient but where it is subnormal; an infinite quotient stays.  Of a subnormal d there may be no reciprocal; it is refused.
 __device__ __forceinline__ float pushed_down(float x, float d, float r) {
   const bool above = x > 0.0f;
   const float q = x * (above ? r : d);
@@ -521,7 +521,7 @@ static int logits_fill(const FrlLogitsDesc* d, const FrlLogitsBufs* b, bool choo
   if (d->history_len > 0 && b->history == nullptr) { set_error("logits: bufs.history is NULL (history_len %d)", d->history_len); return FRL_EINVAL; }
   if (d->n_sparse > 0 && (b->bias_tokens == nullptr || b->bias_values == nullptr)) { set_error("logits: bufs.bias_tokens / bias_values is NULL (n_sparse %d)", d->n_sparse); return FRL_EINVAL; }
   if ((d->mask != FRL_MASK_NONE) != (b->allowed != nullptr)) { set_error("logits: bufs.allowed must be non-NULL exactly when desc.mask is set"); return FRL_EINVAL; }
-  if (d->history_len > 0 && b->repetition == nullptr && !(d->repetition > 0.0f)) { set_error("logits: repetition %g must be > 0", d->repetition); return FRL_EINVAL; }
+  if (d->history_len > 0 && b->repetition == nullptr && !(d->repetition >= 1.17549435e-38f)) { set_error("logits: repetition %g must be > 0 and no subnormal number", d->repetition); return FRL_EINVAL; }
   a = LogitsArgs{b->logits, b->out, b->history, b->lengths, b->prompt_lengths, b->repetition, b->frequency, b->presence,
                  b->bias, b->bias_tokens, b->bias_values, b->allowed, b->temperature, b->gumbel, b->token, b->logprob,
                  nullptr, nullptr, nullptr, nullptr,

@@ -42,7 +42,7 @@ class Constraints:
     history         (rows, L) int32 / int64 tokens so far.  ``lengths`` (rows,) int32: how many of a row's entries are filled (default
                     all); ``prompt_lengths`` (rows,) int32: how many of those are the prompt (default none).  Tokens outside the
                     vocabulary are padding.
-    repetition      > 0: a token seen anywhere in the history has its positive logit divided, its negative one multiplied by it
+    repetition      > 0 (and no subnormal number): a token seen anywhere in the history has its positive logit divided, its negative one multiplied by it
     frequency       subtracted once per time the token was generated (stands behind the prompt)
     presence        subtracted once if it was generated at all
                     (each of the three a number, or a float32 tensor (rows,); without a history they do nothing)

@@ -515,7 +515,7 @@ typedef struct FrlLogitsBufs {
   const void* history;            /* (rows, history_len) tokens */
   const int32_t* lengths;         /* (rows,) or NULL: every row is full */
   const int32_t* prompt_lengths;  /* (rows,) or NULL: no prompt */
-  const float* repetition;        /* (rows,) or NULL; > 0 */
+  const float* repetition;        /* (rows,) or NULL; > 0 and no subnormal number (its reciprocal is taken) */
   const float* frequency;         /* (rows,) or NULL */
   const float* presence;          /* (rows,) or NULL */
   const float* bias;              /* (rows | 1, vocab) or NULL */

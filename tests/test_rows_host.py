@@ -81,3 +81,12 @@ def test_results_that_share_entries_with_logits_are_refused(lib, off, kw):
         b.logits, b.ids, b.teacher, b.loss, b.grad, b.row_stats, b.g_loss = 1 << 30, 1 << 12, 1 << 13, 1 << 14, (1 << 30) + 2 * off, 1 << 16, 1 << 15
         for rc in (lib.frl_distill_fwd(C.byref(d), C.byref(b), 4096, 1 << 30, None), lib.frl_distill_bwd(C.byref(d), C.byref(b), None)):
             assert rc == _lib.FRL_EINVAL and b"overlaps" in lib.frl_last_error()
+
+
+@pytest.mark.parametrize("repetition", [1e-39, 1e-45, 0.0, -1.0, float("nan")])
+def test_repetition_without_a_reciprocal_is_refused(lib, repetition):
+    """1 / 1e-39 is no float32 number: every quotient would be infinite."""
+    d, b = _rows(history_len=3, repetition=repetition), _lib.FrlLogitsBufs()
+    b.logits, b.out, b.history, b.token = 1 << 30, 1 << 40, 1 << 13, 1 << 12
+    assert lib.frl_logits_constrain(C.byref(d), C.byref(b), None) == _lib.FRL_EINVAL and b"repetition" in lib.frl_last_error()
+    assert lib.frl_logits_choose(C.byref(d), C.byref(b), 4096, 1 << 20, None) == _lib.FRL_EINVAL and b"repetition" in lib.frl_last_error()
