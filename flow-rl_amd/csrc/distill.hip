@@ -108,9 +108,23 @@ struct Running {
   }
 };
 
+// The same for the few named entries of a thread, one at a time and without a branch; the reference is m c itself.
+struct Few {
+  float m = -INFINITY, s = 0.0f;
+  __device__ __forceinline__ void about(float all, float c) {
+    const float base = all == -INFINITY ? 0.0f : all;
+    s *= __builtin_amdgcn_exp2f((m - base) * c);
+    m = all;
+  }
+  __device__ __forceinline__ void one(float x, float c) {
+    about(fmaxf(m, x), c);
+    s += __builtin_amdgcn_exp2f((x - (m == -INFINITY ? 0.0f : m)) * c);
+  }
+};
+
 // Named entries among a vector's N: they go into a sum of their own, and -inf takes their place among the rest.  Few vectors have one.
 template <typename T>
-__device__ __forceinline__ void take_named(u32x4& raw, unsigned named, float c, Running& of_named) {
+__device__ __forceinline__ void take_named(u32x4& raw, unsigned named, float c, Few& of_named) {
   const unsigned ninf = Vec16<T>::fill_minus_inf()[0];
   while (named != 0u) {
     const int i = __builtin_ctz(named), w = sizeof(T) == 4 ? i : i >> 1;
@@ -134,7 +148,8 @@ __device__ __forceinline__ void take_named(u32x4& raw, unsigned named, float c, 
 // A thread's share of a row that is streamed
 template <bool REST>
 struct Share {
-  Running run, of_named;                                   // without REST everything is in `run`
+  Running run;                                             // without REST everything is in here
+  Few of_named;
   // vectors [from, to) of the vectors at z, G threads apart; the first one's named bits begin at bit0.  Those before `keep` stay in LDS (at `kept`) for
   // the same thread's gradient.
   template <typename T, int G>
@@ -188,7 +203,7 @@ struct Sums {
       o.m = fmaxf(mr, mn);
       const Shift sh(o.m, c);
       o.down = mr == -INFINITY ? 0.0f : sh.from(Shift(mr, c));
-      o.s = (mr == -INFINITY ? r : r * o.down) + (mn == -INFINITY ? n : n * sh.from(Shift(mn, c)));      // of -inf alone a sum is 0 (or NaN)
+      o.s = (mr == -INFINITY ? r : r * o.down) + (mn == -INFINITY ? n : n * sh.from_exact(mn));      // of -inf alone a sum is 0 (or NaN)
     }
     return o;
   }
@@ -545,7 +560,7 @@ __global__ void __launch_bounds__(1024) frl_distill_join_kernel(const DistillArg
       for (int i = lane; i < a.segs; i += 64) {              // a segment of -inf alone has a sum of 0 (or NaN)
         const f32x4 v = *(const f32x4*)(p + 4 * i);
         r += v[0] == -INFINITY ? v[1] : v[1] * Shift(mr, a.scale2).from(Shift(v[0], a.scale2));
-        n += v[2] == -INFINITY ? v[3] : v[3] * Shift(mn, a.scale2).from(Shift(v[2], a.scale2));
+        n += v[2] == -INFINITY ? v[3] : v[3] * __builtin_amdgcn_exp2f((v[2] - mn) * a.scale2);
       }
       r = wave_reduce<SumOp>(r);
       n = wave_reduce<SumOp>(n);

@@ -167,6 +167,8 @@ struct Shift {
   __device__ __forceinline__ float from(const Shift& o) const {
     return __builtin_amdgcn_exp2f(fast && o.fast ? o.M - M : __builtin_fmaf(o.m - m, c, o.residue() - residue()));
   }
+  // the same for a sum about lower c itself
+  __device__ __forceinline__ float from_exact(float lower) const { return __builtin_amdgcn_exp2f(__builtin_fmaf(lower - m, c, -residue())); }
 };
 
 template <int N>
