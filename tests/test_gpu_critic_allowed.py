@@ -114,3 +114,33 @@ def test_captured_with_a_mask():
         got = [t.clone() for t in out]
         want = fh.critic_select(critic, p, obs, actions, N, temperature=0.5, gumbel=g, allowed=allowed)
         assert all(torch.equal(torch.nan_to_num(a, nan=-9.0), torch.nan_to_num(b, nan=-9.0)) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("T", [0.0, 0.7])
+def test_sample_and_select_with_a_mask(T):
+    """The sampled candidates, chosen from as critic_select chooses: with a mask of everything what it answers without one; builds that have no mask refuse."""
+    import torch
+    import flowrl_hip as fh
+    import helpers as H
+    B, N = 40, 8
+    c = H.Case("allowed", "ddpm", A=3, S=11, T=5, B=B * N, particles=N, seed=11)
+    params, xT, cond, noise = H.make_inputs(c)
+    model = H.product_model(c, params)
+    critic, p = _critic(11, 3)
+    rng = np.random.default_rng(12)
+    obs = torch.from_numpy(cond).cuda()
+    g = torch.from_numpy(rng.gumbel(size=(B, N)).astype(np.float32)).cuda() if T > 0 else None
+    kw = dict(xT=torch.from_numpy(xT.reshape(B, N, 3)).cuda(), noise=torch.from_numpy(noise).cuda(), gumbel=g)
+    allowed = torch.from_numpy(rng.random((B, N)) < 0.5).cuda()
+    allowed[3] = False
+    run = lambda **k: fh.sample_and_select(model, critic, p, None, obs, False, N, "ddpm", T, **kw, **k)[1]  # noqa: E731
+    _, x0, _ = model.sample(None, kw["xT"], obs, False, "ddpm", noise=kw["noise"], particles=N)
+    best = run(allowed=allowed)
+    want, idx, _ = fh.critic_select(critic, p, obs, x0, N, temperature=T, gumbel=g, allowed=allowed)
+    assert idx[3] == -1 and torch.isnan(best[3]).all() and allowed[torch.arange(B, device="cuda"), idx.long()][idx >= 0].all()
+    assert torch.equal(torch.nan_to_num(best, nan=9.0), torch.nan_to_num(want, nan=9.0))
+    assert torch.equal(run(allowed=torch.ones_like(allowed)), run(fused=False))
+    with pytest.raises(fh.FlowRLHipUnsupported, match="allowed"):
+        run(allowed=allowed, fused=True)
+    with pytest.raises(ValueError, match="temperature"):
+        fh.sample_and_select(model, critic, p, None, obs, False, N, "ddpm", None, allowed=allowed, **kw)
