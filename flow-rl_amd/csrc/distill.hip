@@ -381,8 +381,8 @@ __device__ __forceinline__ void keep_packed(u32x4* raw) {
 }
 
 // A row to a group, its first NV vectors per thread held in registers: value, what the backward needs, and (GRAD) the gradient.
-// Bound by HBM: 2048 x 131072 bf16, value: 92 us, 5.8 TB/s of the 5.9 that reads alone reach; 4096 x 32000 bf16 with its gradient: 100 us, 5.2 TB/s;
-// 8192 x 131072 bf16 with named rest and gradient: 881 us, 5.1 TB/s (a large copy: 4.9 to 5.4).  A row's passes (maximum, sum, gradient) wait for
+// Bound by HBM: 2048 x 131072 bf16, value with a rest: 94 us, 5.7 TB/s of the 5.9 that reads alone reach; 4096 x 32000 bf16 with its gradient: 100 us,
+// 5.2 TB/s; 8192 x 131072 bf16 with a rest and its gradient: 888 us, 5.0 TB/s (a large copy: 4.9 to 5.4).  A row's passes (maximum, sum, gradient) wait for
 // one another, so it takes a second workgroup on the CU to keep the memory busy; hence at most 512 threads with what they hold in registers.
 template <typename T, int G, int NV, bool REST, bool GRAD>
 __global__ void __launch_bounds__(G <= 64 ? 256 : G, 4) frl_distill_row_kernel(const DistillArgs a) {

@@ -11,8 +11,10 @@
 // logits, which are on their way meanwhile.  Two sets of words take turns, so a chunk costs one barrier; a choice keeps its maximum and sum in
 // registers from chunk to chunk and reduces them once.
 // Measured: constraining 512 x 131072 f32 with every rule 105 us, 5.2 TB/s of the 5.4 a copy reaches, by HBM; a choice of 256 x 131072 bf16
-// with every rule 50 us, 3.8 TB/s, by vector issue (39 instructions an entry: nearly every wave has a listed entry at nearly every place, so it is
-// the lists' arithmetic that counts; a loop over what each lane has listed instead took 60 us); a few rows 7 us, by the latency of lists, LDS and logits.
+// with every rule 50 us and 4.6 for the join, 3.5 TB/s, mostly by vector issue (40 instructions an entry, 35 of the 50 us: nearly every wave has a
+// listed entry at nearly every place, so it is the lists' arithmetic that counts; a loop over what each lane has listed instead took 60 us);
+// greedy and without lists 24 us and 4.6 for the join, by vector issue (22 instructions an entry, 20 of the 24 us; one of them is the
+// exponential); a few rows 7 us, by the latency of lists, LDS and logits.
 #include "frl_rows.h"
 
 namespace frl {
@@ -438,7 +440,10 @@ struct LogitsPlan { int G, chunks, per, parts; };
 //   choose     300 x 131072   35   / 43    41   / 46    67   / 51    180   / 92
 //   choose    4000 x   5000   39   / 61    46   / 65    68   / 70
 // Over 25 sizes of each operator with five or six histories the calls it picks are 1.17 times as fast (geometric mean; 0.88 to 3.3 times) as with 1024
-// threads wherever lists meet two such workgroups a CU.  Six candidates for the groups of a row, so that choosing costs well under a microsecond.
+// threads wherever lists meet two such workgroups a CU.  The model knows neither the size of an element nor noise: of 512 x 131072 f32 with a history of 4096
+// it expects 46 us and not 105.  What it picks is still near the better of the two: over 108 calls (constrain, greedy and drawn choices, f32 and
+// bf16, six sizes, histories of 0, 256 and 4096, either size forced) 1.01 times its time (geometric mean), 1.12 at the worst (constrain 4000 x
+// 12000 f32, 72 us by 256 and 65 by 1024 threads).  Six candidates for the groups of a row, so that choosing costs well under a microsecond.
 struct GroupCost { float start, start_list, chunk, chunk_list; };
 
 static LogitsPlan logits_plan(const FrlLogitsDesc* d, bool choose) {

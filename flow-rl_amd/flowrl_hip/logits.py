@@ -386,7 +386,8 @@ def distill_loss(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor,
     ``ids`` (rows, top) int32 / int64 (entries outside the vocabulary are padding), ``teacher`` (rows, top), top <= 1024:
       kind "logits"    the teacher's logits; p = softmax(teacher / temperature) over the named entries
       kind "logprobs"  its log-probabilities (at the temperature meant); what they leave of 1 is one more class, "the rest", which
-                       the student fills with all entries that are not named
+                       the student fills with all entries that are not named (a teacher that names the whole vocabulary leaves none:
+                       its log-probabilities times the temperature go as "logits")
     ``weights`` (rows,) float32: a row of weight 0 is not read.  ``reduction`` "mean" divides by the sum of the weights; "none" returns
     the rows' weighted divergences.  With ``want_grad`` also d loss / d logits in the logits' type, in the same pass ("none": of
     the rows' sum).  Like ``mse_loss`` a value without a graph; :func:`flowrl_hip.autograd.distill_loss` differentiates."""

@@ -547,6 +547,8 @@ int frl_logits_choose(const FrlLogitsDesc* desc, const FrlLogitsBufs* bufs, void
  *   FRL_DISTILL_REST  teacher holds log-probabilities (at the temperature meant): p = exp(teacher), and the mass it leaves
  *                     unnamed, P = 1 - sum p, is one more class of which the student has Q = the sum of q over the others:
  *                     L[r] = sum p (log p - log q) + P log(P / Q)          (the last term only where P > 0)
+ * (a teacher that names the whole vocabulary leaves no entry for such mass, and rounded log-probabilities hardly sum to 1: give them, times
+ * the temperature, as FRL_DISTILL_TOP, which renormalises).  Only a rest of no entry, or of -inf alone, has Q = 0: L is infinite there, the rest's gradient 0.
  * A token named twice counts as two entries (their p add up in the gradient; Q leaves it out once).  A row that names
  * nothing under FRL_DISTILL_TOP, and a row of weight 0 (never read), have L = 0 and gradient 0.
  *   loss, FRL_REDUCE_NONE: (rows,) weights[r] L[r];  FRL_REDUCE_SUM: their sum;  FRL_REDUCE_MEAN: their sum / the sum of the
