@@ -210,8 +210,8 @@ struct Sums {
 };
 
 // What W lanes make of a row's teacher entries: the tokens (into sid, -1 for padding), p (into sp, 0 for padding) and their logits (into sz),
-// sum p, the largest of their logits and sum p (log p + (largest - z) / T).  The three loads of an entry are under way together; what follows works on LDS.  FRL_DISTILL_REST needs
-// 1 - sum p, which float32 exponentials would leave without digits: float64.
+// sum p, the largest of their logits and sum p (log p + (largest - z) / T).  The three loads of an entry are under way together; what follows
+// works on LDS.  FRL_DISTILL_REST needs 1 - sum p, which float32 exponentials would leave without digits: float64.
 template <typename T, int W, bool REST>
 __device__ __forceinline__ void teacher_part(const DistillArgs& a, long long row, const T* z, int lane, int* sid, float* sp, float* sz, double& sum_p, double& cross, float& largest) {
   sum_p = cross = 0.0;

@@ -164,3 +164,34 @@ def test_a_rest_of_nothing(N, V, K, dtype):
         assert float(got[1]) == float("inf") and torch.isfinite(got[torch.arange(N, device="cuda") != 1]).all()
     _check_gradients(grads, pick, g, tolg)
     assert not any(got[1].cpu()[~named[1]].any() for got in grads)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("skip,gap", [(0, 0), (1, 2), (3, 1), (7, 4)])
+@pytest.mark.parametrize("N,V", [(4, 61), (5, 1003), (260, 9001), (3, 50001), (257, 70001)])
+def test_named_ends_and_repeats_far_above_the_rest(N, V, skip, gap, dtype):
+    """Rows that start anywhere: the single entries before and behind the vectors are named, some of them twice, and lie far above the rest."""
+    import torch
+    import flowrl_hip as fh
+    rng = np.random.default_rng(V + skip)
+    K, dt = 24, getattr(torch, dtype)
+    z, ids, t = make_distill(rng, N, V, K, "logprobs", dt, repeats=True)
+    ids[:, :8] = np.arange(8)
+    ids[:, 8:16] = V - 1 - np.arange(8)
+    ids[:, 16:18] = [0, V - 1]
+    t -= 1.0                                             # a token named several times counts as often: mass is left all the same
+    z.scatter_(1, torch.from_numpy(ids).long(), torch.from_numpy((200.0 + rng.standard_normal((N, K))).astype(np.float32)).to(dt))
+    buf = torch.zeros((N * (V + gap) + skip,), dtype=dt, device="cuda")
+    view = buf[skip:].view(N, V + gap)[:, :V]
+    view.copy_(z)
+    pick = _picked(N)
+    L, g, tolL, tolg = rows_of(z[pick], ids[pick], t[pick], "logprobs", 1.0)
+    args = (torch.from_numpy(ids).cuda(), torch.from_numpy(t).cuda())
+    kw = dict(kind="logprobs", reduction="none")
+    rows, grad = fh.logits.distill_loss(view, *args, want_grad=True, **kw)
+    value = fh.logits.distill_loss(view, *args, **kw)
+    leaf = view.detach().requires_grad_(True)
+    out = fh.autograd.distill_loss(leaf, *args, **kw)
+    back, = torch.autograd.grad(out, leaf, torch.ones_like(out))
+    _check_losses((rows, value, out.detach()), pick, L, tolL)
+    _check_gradients((grad, back), pick, g, tolg)
