@@ -26,8 +26,8 @@ ARCH = "gfx950"
 NO_PACKED = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # (source, object stem, extra defines); the register-streamed sampler is one translation unit per activation
 SOURCES = [("capi.hip", "capi", []), ("prepare.hip", "prepare", []),
-           ("cond_embed.hip", "cond_embed", []), ("critic_select.hip", "critic_select", []), ("time_bwd.hip", "time_bwd", []), ("rng.hip", "rng", []), ("net_eval.hip", "net_eval", []), ("net_vjp_layered.hip", "net_vjp_layered", []),
-           # rows of logits: scalar float32 throughout (the packed forms buy a memory-bound kernel nothing)
+           ("cond_embed.hip", "cond_embed", []), ("critic_select.hip", "critic_select", NO_PACKED), ("time_bwd.hip", "time_bwd", []), ("rng.hip", "rng", []), ("net_eval.hip", "net_eval", []), ("net_vjp_layered.hip", "net_vjp_layered", []),
+           # rows of logits (and the selection above): scalar float32 throughout (the packed forms buy a memory-bound kernel nothing)
            ("logits.hip", "logits", NO_PACKED), ("distill.hip", "distill", NO_PACKED),
            ("sampler_bf16.hip", "sampler_bf16", ["-fno-slp-vectorize"]),
            ] + [("sampler_bwd_bf16.hip", f"sampler_bwd_bf16_p{p}", ["-fno-slp-vectorize", f"-DFRL_BWD16_PHASE={p}"]) for p in range(3)] + \
